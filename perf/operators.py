@@ -499,8 +499,12 @@ def exact(case, seed):
         key = s["key"].double() if s["frequencies"] is None else _turned(s["key"], s, c, 1.0)
         for name, x in (("key", key), ("value", s["value"].double())):
             groups = x.unflatten(-1, (-1, g))
-            step = torch.maximum(groups.amax(-1), -groups.amin(-1)).clamp_min(1e-8) / (mid - 1.0)
-            level = torch.clamp(torch.round(groups / step[..., None]), -mid, mid - 1)
+            # the format's quantizer rounds the step and the quotient to FP32 (16-bit inputs hit
+            # the border between two codes exactly, so these roundings belong to the definition)
+            step = torch.maximum(groups.amax(-1), -groups.amin(-1)).float().double().clamp_min(1e-8)
+            step = torch.true_divide(step, torch.full_like(step, mid - 1.0)).float().double()
+            level = torch.round((groups.float().double() / step[..., None]).float().double())
+            level = torch.clamp(level, -mid, mid - 1)
             held = step.half().double()  # scales are FP16 by the cache's format
             out[name] = (level * held[..., None]).flatten(-2)
             pool = torch.zeros(s["scales_" + name[0]].shape, dtype=torch.float64, device=x.device)
