@@ -270,7 +270,7 @@ def _prepare_weights(case, gen):
          "sm_scale": 1.0 / math.sqrt(d)}
     if case["lse"]:  # what the step's attention has returned beside its output
         scores = _scores({"case": case, **s})
-        s["lse"] = torch.logsumexp(scores.double(), -1).float()
+        s["lse"] = torch.logsumexp(scores.double(), -1).float().transpose(0, 1).reshape(tq, qh)
     return s
 
 
@@ -371,7 +371,7 @@ def _plain_weights(s):
         top = torch.where(top == -math.inf, 0.0, top)
         lse = (scores - top).exp_().sum(-1).log() + top.squeeze(-1)
     else:
-        lse = s["lse"]
+        lse = s["lse"].reshape(c["queries"], c["kv_heads"], -1).transpose(0, 1)
     empty = lse == -math.inf
     p = (scores - torch.where(empty, 0.0, lse).unsqueeze(-1)).exp_()
     return s["previous"] + p.sum((1, 2)), lse.transpose(0, 1).reshape(c["queries"], c["heads"])
