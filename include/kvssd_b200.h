@@ -364,6 +364,103 @@ KVSSD_B200_API int kvssd_b200_dequantize(const uint8_t* packed, const uint16_t* 
                           int head_dim, int bits, int group_size, int mode, uint16_t* values,
                           uint8_t* codes, kvssd_b200_stream_t stream);
 
+/* Cache maintenance around the decode: rotary positions, the quantizing cache write, the attention
+ * weight each cached token gets, and eviction by it. Index arrays are int32, or int64 where the
+ * argument beside them is nonzero; strides are in elements and the last dimension is contiguous;
+ * `device_status` (NULL, or the status word of a workspace: see kvssd_b200_read_status) is OR-ed with
+ * 1 for a slot or block-table entry outside the pool (skipped) and 2 for a valid count outside
+ * [0, block_tokens] (clamped). Calls of one operator share no state: they may overlap on several
+ * streams as long as their buffers differ. head_dim is at most 256. */
+
+/* Rotary positions of x [tokens, heads, head_dim] (KVSSD_B200_Q_F32 / _F16 / _BF16) into `out` of the
+ * same shape and type, which may be x itself (with its strides) and else must not overlap it. Of the
+ * first 2 * pairs dims of a head, pair i = (a, b) -- dims i and i + pairs, or 2i and 2i + 1 when
+ * `interleaved` -- becomes magnitude * (a cos t - b sin t, b cos t + a sin t) with
+ * t = positions[token] * frequencies[i] (FP64); the dims behind are copied. No reference
+ * counterpart (the reference caches keys as it is given them, src/kvssd/store.py:27-67). */
+KVSSD_B200_API int kvssd_b200_rotary(const void* x, int dtype, long long x_token_stride,
+                      long long x_head_stride, int tokens, int heads, int head_dim,
+                      const void* positions, int positions_int64, const double* frequencies,
+                      int pairs, int interleaved, float magnitude, void* out,
+                      long long out_token_stride, long long out_head_stride,
+                      kvssd_b200_stream_t stream);
+
+/* Quantizes the keys and values [tokens, kv_heads, head_dim] of `tokens` tokens into their slots of a
+ * block pool: token i goes to row slots[i] % block_tokens of block slots[i] / block_tokens; a
+ * negative slot is skipped (padding). The slots of one call must differ from each other (of two
+ * equal ones the row holds a mixture). With `frequencies` (else NULL) the keys are rotated first, as
+ * kvssd_b200_rotary does but rounded to FP32 once and not to their type. Codes and scales are those
+ * of quantize_tensor (src/kvssd/quant.py:49-65), bit for bit, as KVCacheStore.create stores them
+ * (src/kvssd/store.py:50-59); a NaN makes its group's scale NaN. Where `valid_tokens` is not NULL the
+ * counts of the written blocks are raised to cover the written rows. key_values and value_values
+ * (both or neither NULL) receive the FP16 values that the cache now holds for the tokens,
+ * [tokens, kv_heads, head_dim] (dequantize_tensor, src/kvssd/quant.py:68-73), skipped tokens
+ * included. */
+KVSSD_B200_API int kvssd_b200_append(const void* key, const void* value, int dtype,
+                      long long key_token_stride, long long key_head_stride,
+                      long long value_token_stride, long long value_head_stride, int tokens,
+                      const void* slots, int slots_int64, const void* positions,
+                      int positions_int64, const double* frequencies, int pairs, int interleaved,
+                      float magnitude, uint8_t* packed_k, uint8_t* packed_v, uint16_t* scales_k,
+                      uint16_t* scales_v, int32_t* valid_tokens, int n_pool_blocks,
+                      int block_tokens, int kv_heads, int head_dim, int bits, int group_size,
+                      uint16_t* key_values, uint16_t* value_values, unsigned* device_status,
+                      kvssd_b200_stream_t stream);
+
+/* Bytes of device scratch kvssd_b200_attention_weights needs when it computes the log-sum-exps
+ * (none otherwise; its contents need not be kept or cleared). No reference counterpart. */
+KVSSD_B200_API int kvssd_b200_attention_weights_scratch_size(int queries, int n_sel_blocks,
+                      int block_tokens, int query_heads, int kv_heads, int head_dim, int bits,
+                      int group_size, size_t* bytes);
+
+/* The attention weight of every selected place: for KV head h and place i (row i % block_tokens of
+ * selected block i / block_tokens)
+ *   out[h, i] = previous[h, i] + sum over the queries t and the query heads g of h of
+ *               exp(sm_scale * q[t, g] . k[i, h] - lse[t, g]),
+ * with previous = NULL for zero; `out` may be `previous` (with its stride) and else must not overlap
+ * it. query [queries, query_heads, head_dim]; a place counts for query t when its row lies before
+ * the block's valid count and i < visible[t] (NULL: all). lse [queries, query_heads]: given
+ * (lse_given nonzero, as kvssd_b200_decode returns it), or computed and written (-inf for a query
+ * that sees nothing, which then adds nothing). Blocks may be selected several times. Each output
+ * is summed in a fixed order. No reference counterpart (the reference selects blocks by their
+ * order only, src/kvssd/selectors.py:11-28). */
+KVSSD_B200_API int kvssd_b200_attention_weights(const void* query, int query_dtype, int queries,
+                      const uint8_t* packed_k, const uint16_t* scales_k,
+                      const int32_t* valid_tokens, const int32_t* block_table,
+                      const int32_t* visible, int n_pool_blocks, int n_sel_blocks,
+                      int block_tokens, int query_heads, int kv_heads, int head_dim, int bits,
+                      int group_size, float sm_scale, int lse_given, float* lse,
+                      const float* previous, long long previous_stride, float* out,
+                      long long out_stride, void* scratch, size_t scratch_bytes,
+                      unsigned* device_status, kvssd_b200_stream_t stream);
+
+/* Bytes of device scratch kvssd_b200_evict needs (contents need not be kept or cleared). No
+ * reference counterpart. */
+KVSSD_B200_API int kvssd_b200_evict_scratch_size(int n_tokens, int keep, int kv_heads, int shared,
+                      size_t* bytes);
+
+/* Compacts a cache of n_tokens tokens (places 0 .. n_tokens - 1 of the selected blocks, in order) to
+ * `keep` of them, chosen by each KV head, or by all together when `shared` (by the sum of the heads'
+ * weights in FP64, rounded to FP32; the positions of head 0 count): tokens whose position is below
+ * `sink` or at least `recent_from`, then those of the largest weight; equal weights go by the lower
+ * place, a NaN ranks last, more than `keep` protected tokens go by the lower place too. The j-th
+ * place below `keep` that was given up (in order) receives the j-th kept token from behind `keep`:
+ * its packed row and scales in place (the rows from `keep` on are left as they were), its weight
+ * and position in new_weights and new_positions [kv_heads, columns], which hold 0 and -1 from `keep`
+ * on and must not overlap the inputs weights and positions (row strides as given). valid_tokens of
+ * the selected blocks becomes the rows they still hold. Block-table entries must differ from each
+ * other. A pool row has packed_dim bytes of codes and `groups` scales a head, K and V alike. No
+ * reference counterpart (the reference selects whole blocks by their order,
+ * src/kvssd/selectors.py:17-28). */
+KVSSD_B200_API int kvssd_b200_evict(const float* weights, long long weights_stride,
+                      const int32_t* positions, long long positions_stride, int n_tokens, int keep,
+                      int sink, long long recent_from, int shared, float* new_weights,
+                      int32_t* new_positions, int columns, uint8_t* packed_k, uint8_t* packed_v,
+                      uint16_t* scales_k, uint16_t* scales_v, int32_t* valid_tokens,
+                      const int32_t* block_table, int n_pool_blocks, int n_sel_blocks,
+                      int block_tokens, int kv_heads, int packed_dim, int groups, void* scratch,
+                      size_t scratch_bytes, unsigned* device_status, kvssd_b200_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

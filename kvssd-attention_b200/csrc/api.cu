@@ -254,6 +254,9 @@ cudaError_t launch_combine(const float* part_acc, const float* part_ml, int n_pa
 }
 
 }  // namespace
+
+int report(int status, const char* message) { return fail(status, message); }
+
 }  // namespace kvb
 
 using namespace kvb;

@@ -1,0 +1,165 @@
+// Cache-maintenance operators around the decode attention: rotary positions (rotary.cu), the
+// quantizing cache write (append.cu), attention weights over the packed keys (weights.cu) and
+// eviction by them (evict.cu). Launch arguments, the functions cache_api.cu calls, and the device
+// helpers the kernels share.
+//
+// Every kernel is launched with programmatic stream serialization: its first instruction that
+// touches global memory comes after pdl_wait().
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "common.cuh"
+
+namespace kvb {
+
+// A [tokens, heads, head_dim] tensor: strides in elements, the last dimension contiguous.
+struct RowTensor {
+  const void* p;
+  long long token, head;
+};
+
+// int32 or int64 indices.
+struct Indices {
+  const void* p;
+  int wide;  // 1: int64
+};
+
+struct RotaryArgs {
+  RowTensor x;
+  void* out;
+  long long out_token, out_head;
+  int dtype;
+  int tokens, heads, d;
+  Indices positions;
+  const double* freq;  // radians a position, [pairs]
+  int pairs, interleaved;
+  float magnitude;
+};
+
+struct AppendArgs {
+  RowTensor key, value;
+  int dtype;
+  int tokens;
+  Indices slots, positions;
+  const double* freq;  // nullptr: keys are stored as they are
+  int pairs, interleaved;
+  float magnitude;
+  uint8_t* packed[2];  // K, V
+  __half* scales[2];
+  __half* values[2];   // nullptr, or FP16 [tokens, kvh, d]
+  int32_t* valid;      // nullptr, or [n_pool]
+  int n_pool, bt, kvh, d, bits, group;
+  unsigned* status;    // nullptr, or the sticky status word
+};
+
+struct WeightsArgs {
+  const void* query;
+  int dtype;
+  int queries, qh;
+  const uint8_t* kp;
+  const __half* ks;
+  const int32_t* valid;
+  const int32_t* table;    // nullptr: slots 0 .. n_sel - 1
+  const int32_t* visible;  // nullptr: every query sees every place
+  int n_pool, n_sel, bt, kvh, d, bits, group;
+  float sm_scale;
+  const float* lse_in;     // nullptr: computed
+  float* lse;              // [queries, qh], written when computed
+  const float* previous;   // nullptr, or [kvh, n_sel * bt] with this row stride
+  long long previous_stride;
+  float* out;
+  long long out_stride;
+  float* scratch;          // parts of the log-sum-exps when computed
+  unsigned* status;
+};
+
+struct EvictArgs {
+  const float* weights;
+  long long weights_stride;
+  const int32_t* positions;
+  long long positions_stride;
+  int n, keep, columns;    // columns of the outputs
+  int sink;                // positions below are kept
+  long long recent_from;   // positions from here on are kept
+  int shared;
+  float* new_weights;      // [kvh, columns]
+  int32_t* new_positions;  // [kvh, columns]
+  int32_t* holes;          // scratch [lists, keep]
+  int32_t* movers;         // scratch [lists, n - keep]
+  int32_t* counts;         // scratch [lists]
+  uint8_t* packed[2];
+  __half* scales[2];
+  int32_t* valid;
+  const int32_t* table;
+  int n_pool, n_sel, bt, kvh;
+  int packed_dim, groups;  // bytes of codes and scales of one (token, head)
+  unsigned* status;
+};
+
+// Sets the calling thread's last error and returns `status` (api.cu).
+int report(int status, const char* message);
+
+cudaError_t launch_rotary(const RotaryArgs& a, cudaStream_t s);
+cudaError_t launch_append(const AppendArgs& a, cudaStream_t s);
+size_t weights_scratch_bytes(int queries, int qh, int n_sel, int bt);
+cudaError_t launch_weights(const WeightsArgs& a, cudaStream_t s);
+cudaError_t launch_evict(const EvictArgs& a, cudaStream_t s);
+
+// Launch with programmatic stream serialization (see above).
+template <typename... Params, typename... Given>
+cudaError_t launch_pdl(void (*kernel)(Params...), dim3 grid, int threads, size_t smem,
+                       cudaStream_t s, Given... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, Params(args)...);
+}
+
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_launch() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+__device__ __forceinline__ long long index_at(const Indices& ix, long long i) {
+  return ix.wide ? static_cast<const long long*>(ix.p)[i] : static_cast<const int32_t*>(ix.p)[i];
+}
+
+// Element types of the rotary and append operators.
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float x);
+template <>
+__device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) {
+  return __float2bfloat16_rn(x);
+}
+
+// The angle of `position` at `freq` radians a position, as a fraction of a turn in [-1/2, 1/2].
+// The angle is the FP64 product; its division by 2 pi keeps the product's low part (1 / (2 pi) as
+// a pair of doubles), so a far position loses nothing against reducing the FP64 angle exactly.
+__device__ __forceinline__ double turn_fraction(long long position, double freq) {
+  constexpr double kInv2PiHi = 0.15915494309189535;        // fl64(1 / (2 pi))
+  constexpr double kInv2PiLo = -9.839338337591243e-18;     // 1 / (2 pi) - kInv2PiHi
+  const double angle = static_cast<double>(position) * freq;
+  const double hi = angle * kInv2PiHi;
+  const double lo = fma(angle, kInv2PiHi, -hi) + angle * kInv2PiLo;
+  return (hi - rint(hi)) + lo;
+}
+
+}  // namespace kvb

@@ -21,10 +21,12 @@ from .backends import (
     register_attention_backend,
     resolve_attention_backend,
 )
+from .cache import DeviceKVCache
 from .format import CacheSpec
 from .pipeline import KVSSDPipeline
 from .pool import DeviceBlockPool
 from .quant import dequantize_tensor, quantize_tensor
+from .rotary import RotaryEmbedding
 from .selectors import AllBlocks, RecentSinkBlocks
 from .storage import (
     GDSStorageBackend,
@@ -41,11 +43,13 @@ __all__ = [
     "B200AttentionBackend",
     "CacheSpec",
     "DeviceBlockPool",
+    "DeviceKVCache",
     "GDSStorageBackend",
     "KVCacheStore",
     "KVSSDPipeline",
     "PackedBatch",
     "RecentSinkBlocks",
+    "RotaryEmbedding",
     "StorageAvailability",
     "StorageBackend",
     "available_storage_backends",

@@ -132,6 +132,52 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         _c_int,
         [_c_void, _c_void, _c_ll, _c_int, _c_int, _c_int, _c_int, _c_void, _c_void, _c_void],
     ),
+    "kvssd_b200_rotary": (
+        _c_int,
+        [
+            _c_void, _c_int, _c_ll, _c_ll, _c_int, _c_int, _c_int,  # x
+            _c_void, _c_int, _c_void, _c_int, _c_int, _c_float,  # positions, frequencies
+            _c_void, _c_ll, _c_ll, _c_void,  # out, stream
+        ],
+    ),
+    "kvssd_b200_append": (
+        _c_int,
+        [
+            _c_void, _c_void, _c_int, _c_ll, _c_ll, _c_ll, _c_ll, _c_int,  # key, value
+            _c_void, _c_int,  # slots
+            _c_void, _c_int, _c_void, _c_int, _c_int, _c_float,  # positions, frequencies
+            _c_void, _c_void, _c_void, _c_void, _c_void,  # pool
+            _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,  # n_pool, bt, kvh, d, bits, group
+            _c_void, _c_void, _c_void, _c_void,  # values, status, stream
+        ],
+    ),
+    "kvssd_b200_attention_weights_scratch_size": (
+        _c_int, [_c_int] * 8 + [ctypes.POINTER(_c_size)]
+    ),
+    "kvssd_b200_attention_weights": (
+        _c_int,
+        [
+            _c_void, _c_int, _c_int,  # query
+            _c_void, _c_void, _c_void, _c_void, _c_void,  # keys, scales, valid, table, visible
+            _c_int, _c_int, _c_int,  # n_pool, n_sel, block_tokens
+            _c_int, _c_int, _c_int, _c_int, _c_int,  # qh, kvh, d, bits, group
+            _c_float, _c_int, _c_void,  # sm_scale, lse
+            _c_void, _c_ll, _c_void, _c_ll,  # previous, out
+            _c_void, _c_size, _c_void, _c_void,  # scratch, status, stream
+        ],
+    ),
+    "kvssd_b200_evict_scratch_size": (_c_int, [_c_int] * 4 + [ctypes.POINTER(_c_size)]),
+    "kvssd_b200_evict": (
+        _c_int,
+        [
+            _c_void, _c_ll, _c_void, _c_ll,  # weights, positions
+            _c_int, _c_int, _c_int, _c_ll, _c_int,  # n_tokens, keep, sink, recent_from, shared
+            _c_void, _c_void, _c_int,  # new weights and positions
+            _c_void, _c_void, _c_void, _c_void, _c_void, _c_void,  # pool, block table
+            _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,  # geometry
+            _c_void, _c_size, _c_void, _c_void,  # scratch, status, stream
+        ],
+    ),
 }
 
 _lock = threading.Lock()

@@ -653,5 +653,325 @@ def dequantize_packed(
     return codes.reshape(shape), values.reshape(shape)
 
 
+# --- cache maintenance: rotary positions, the quantizing cache write, attention weights, eviction ---
+
+_ELEMENT_DTYPES = {torch.float32: _native.Q_F32, torch.float16: _native.Q_F16,
+                   torch.bfloat16: _native.Q_BF16}
+_INDEX_DTYPES = {torch.int32: 0, torch.int64: 1}
+
+
+def _call(device: torch.device, name: str, *args) -> None:
+    """Calls an entry point with ``device`` current."""
+    fn = getattr(_native.library(), name)
+    if torch.cuda.current_device() == device.index:
+        status = fn(*args)
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args)
+    if status:
+        _native.check(status, name)
+
+
+def _cuda_device(name: str, t: torch.Tensor) -> torch.device:
+    if t.device.type != "cuda":
+        raise RuntimeError(f"{name} requires a CUDA device, got {t.device}")
+    return t.device
+
+
+def _status_word(device: torch.device, stream: int) -> int | None:
+    """Address of the stream's sticky status word (read_device_status, status_watch); None during a
+    graph capture on a stream that has none yet, since creating it would be captured."""
+    ws = _workspaces._buffers.get((device.index, stream))
+    if ws is None:
+        if torch.cuda.is_current_stream_capturing():
+            return None
+        ws = _workspaces.get(device, torch.cuda.current_stream(device), _WORKSPACE_HEADER)
+    return ws.data_ptr()
+
+
+def _require_rows(name: str, t: torch.Tensor, shape, dtype, device) -> None:
+    """A [tokens, heads, head_dim] tensor whose last dimension is contiguous."""
+    if t.device != device or t.dtype != dtype or tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must be {tuple(shape)} {dtype} on {device}, got "
+                         f"{tuple(t.shape)} {t.dtype} on {t.device}")
+    if t.stride(2) != 1 and t.shape[2] > 1:
+        raise ValueError(f"{name} must be contiguous along its last dimension")
+
+
+def _index_kind(name: str, t: torch.Tensor, n: int, device) -> int:
+    kind = _INDEX_DTYPES.get(t.dtype)
+    if kind is None or t.shape != (n,) or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous int32 or int64 [{n}] on {device}, got "
+                         f"{tuple(t.shape)} {t.dtype} on {t.device}")
+    return kind
+
+
+def _check_frequencies(frequencies: torch.Tensor, head_dim: int, device) -> int:
+    if (frequencies.dtype != torch.float64 or frequencies.ndim != 1
+            or frequencies.device != device or not frequencies.is_contiguous()):
+        raise ValueError(f"frequencies must be contiguous float64 [pairs] on {device}")
+    pairs = frequencies.shape[0]
+    if pairs < 1 or 2 * pairs > head_dim:
+        raise ValueError("frequencies must hold 1 to head_dim / 2 pairs")
+    return pairs
+
+
+def rotary(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, *,
+           interleaved: bool = False, magnitude: float = 1.0,
+           out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotary positions of ``x`` [tokens, heads, head_dim] (FP32, FP16 or BF16; any token and head
+    strides), in a new tensor or in ``out``, which may be ``x`` itself.
+
+    ``positions`` int32 or int64 [tokens]; ``frequencies`` float64 [pairs], radians a position (see
+    rotary.RotaryEmbedding for the usual scalings). The first 2 * pairs dims of a head are rotated
+    -- pair i is dims (i, i + pairs), or (2i, 2i + 1) when ``interleaved`` --, the dims behind are
+    copied. Angles are FP64, products FP32, rounded once."""
+    device = _cuda_device("rotary", x)
+    dtype = _ELEMENT_DTYPES.get(x.dtype)
+    if dtype is None:
+        raise ValueError(f"unsupported element type {x.dtype}")
+    if x.ndim != 3:
+        raise ValueError("x must be [tokens, heads, head_dim]")
+    tokens, heads, d = x.shape
+    if x.stride(2) != 1 and out is None:
+        x = x.contiguous()
+    _require_rows("x", x, x.shape, x.dtype, device)
+    kind = _index_kind("positions", positions, tokens, device)
+    pairs = _check_frequencies(frequencies, d, device)
+    if out is None:
+        out = torch.empty((tokens, heads, d), dtype=x.dtype, device=device)
+    else:
+        _require_rows("out", out, x.shape, x.dtype, device)
+        near, far = sorted(((out.stride(0), tokens), (out.stride(1), heads)))
+        if (near[1] > 1 and near[0] < d) or (far[1] > 1 and far[0] < max(near[0] * near[1], d)):
+            raise ValueError("out must not overlap itself")
+    _call(device, "kvssd_b200_rotary", x.data_ptr(), dtype, x.stride(0), x.stride(1), tokens, heads,
+          d, positions.data_ptr(), kind, frequencies.data_ptr(), pairs, interleaved, magnitude,
+          out.data_ptr(), out.stride(0), out.stride(1), _stream_handle(device))
+    return out
+
+
+def _check_pool(packed_k, packed_v, scales_k, scales_v, valid_tokens, bits, group_size, device):
+    """Checks the tensors of a block pool; returns (n_pool, block_tokens, kv_heads, head_dim)."""
+    for name, t, dt in (("packed_k", packed_k, torch.uint8), ("packed_v", packed_v, torch.uint8),
+                        ("scales_k", scales_k, torch.float16),
+                        ("scales_v", scales_v, torch.float16),
+                        ("valid_tokens", valid_tokens, torch.int32)):
+        if t is not None:
+            _require_cuda(name, t, device, dt)
+    if bits not in (2, 4):
+        raise ValueError("bits must be 2 or 4")
+    if packed_k.ndim != 4 or (packed_v is not None and packed_v.shape != packed_k.shape):
+        raise ValueError("packed KV must match [blocks,tokens,kv_heads,packed_dim]")
+    n_pool, bt, kvh, pd = packed_k.shape
+    d = pd * 8 // bits
+    if group_size < 1 or d % group_size:
+        raise ValueError("group_size must divide head_dim")
+    shape = (n_pool, bt, kvh, d // group_size)
+    if scales_k.shape != shape or (scales_v is not None and scales_v.shape != shape):
+        raise ValueError("KV scales must match [blocks,tokens,kv_heads,groups]")
+    if valid_tokens is not None and valid_tokens.shape != (n_pool,):
+        raise ValueError("valid_tokens must contain one count per block")
+    return n_pool, bt, kvh, d
+
+
+def append(key: torch.Tensor, value: torch.Tensor, slots: torch.Tensor, packed_k: torch.Tensor,
+           packed_v: torch.Tensor, scales_k: torch.Tensor, scales_v: torch.Tensor, bits: int,
+           group_size: int, *, positions: torch.Tensor | None = None,
+           frequencies: torch.Tensor | None = None, interleaved: bool = False,
+           magnitude: float = 1.0, valid_tokens: torch.Tensor | None = None,
+           values: bool = False) -> tuple[torch.Tensor, torch.Tensor] | None:
+    """Quantizes the keys and values [tokens, kv_heads, head_dim] (FP32, FP16 or BF16; any token and
+    head strides) of ``tokens`` tokens into their slots of a block pool, in place.
+
+    ``slots`` int32 or int64 [tokens]: block * block_tokens + row; a negative slot is skipped
+    (padding), one behind the pool is skipped and flagged (read_device_status bit 1). The slots of
+    one call must differ from each other. With ``frequencies`` and ``positions`` the keys are rotated
+    first (as ``rotary``, but rounded to FP32 once instead of to their type). Codes and scales equal
+    quant.quantize_tensor's bit for bit. ``valid_tokens`` (optional): the counts of the written
+    blocks are raised to cover the written rows. ``values=True`` returns the FP16 keys and values that
+    the cache now holds for the tokens ([tokens, kv_heads, head_dim], skipped tokens included), for a
+    prompt's own attention to see what later decodes will see."""
+    device = _cuda_device("append", key)
+    dtype = _ELEMENT_DTYPES.get(key.dtype)
+    if dtype is None:
+        raise ValueError(f"unsupported element type {key.dtype}")
+    if key.ndim != 3:
+        raise ValueError("key must be [tokens, kv_heads, head_dim]")
+    n_pool, bt, kvh, d = _check_pool(packed_k, packed_v, scales_k, scales_v, valid_tokens, bits,
+                                     group_size, device)
+    tokens = key.shape[0]
+    _require_rows("key", key, (tokens, kvh, d), key.dtype, device)
+    _require_rows("value", value, (tokens, kvh, d), key.dtype, device)
+    slot_kind = _index_kind("slots", slots, tokens, device)
+    pos_kind = pairs = 0
+    if frequencies is not None:
+        if positions is None:
+            raise ValueError("rotated keys need positions")
+        pos_kind = _index_kind("positions", positions, tokens, device)
+        pairs = _check_frequencies(frequencies, d, device)
+    held = None
+    if values:
+        held = (torch.empty((tokens, kvh, d), dtype=torch.float16, device=device),
+                torch.empty((tokens, kvh, d), dtype=torch.float16, device=device))
+    stream = _stream_handle(device)
+    _call(device, "kvssd_b200_append", key.data_ptr(), value.data_ptr(), dtype, key.stride(0),
+          key.stride(1), value.stride(0), value.stride(1), tokens, slots.data_ptr(), slot_kind,
+          None if pairs == 0 else positions.data_ptr(), pos_kind,
+          None if pairs == 0 else frequencies.data_ptr(), pairs, interleaved, magnitude,
+          packed_k.data_ptr(), packed_v.data_ptr(), scales_k.data_ptr(), scales_v.data_ptr(),
+          _ptr(valid_tokens), n_pool, bt, kvh, d, bits, group_size,
+          None if held is None else held[0].data_ptr(),
+          None if held is None else held[1].data_ptr(), _status_word(device, stream), stream)
+    return held
+
+
+def _check_table(block_table, n_pool: int, device) -> int:
+    if block_table is None:
+        return n_pool
+    _require_cuda("block_table", block_table, device, torch.int32)
+    if block_table.ndim != 1:
+        raise ValueError("block_table must be 1-D")
+    return block_table.shape[0]
+
+
+def _require_stats(name: str, t: torch.Tensor, kvh: int, columns: int | None, dtype, device) -> None:
+    """A [kv_heads, columns] tensor with contiguous rows."""
+    if t.device != device or t.dtype != dtype or t.ndim != 2 or t.shape[0] != kvh or (
+            columns is not None and t.shape[1] != columns):
+        raise ValueError(f"{name} must be [{kvh}, {columns or 'places'}] {dtype} on {device}, got "
+                         f"{tuple(t.shape)} {t.dtype} on {t.device}")
+    if t.shape[1] > 1 and t.stride(1) != 1 or (kvh > 1 and t.stride(0) < t.shape[1]):
+        raise ValueError(f"{name} must have contiguous rows that do not overlap")
+
+
+def attention_weights(query: torch.Tensor, packed_k: torch.Tensor, scales_k: torch.Tensor,
+                      valid_tokens: torch.Tensor, bits: int, group_size: int, sm_scale: float, *,
+                      lse: torch.Tensor | None = None, block_table: torch.Tensor | None = None,
+                      visible: torch.Tensor | None = None, previous: torch.Tensor | None = None,
+                      out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The attention weight every selected place gets: returns (weights fp32
+    [kv_heads, n_sel * block_tokens], lse).
+
+    weights[h, i] = previous[h, i] + the sum over the queries t and the query heads g of KV head h of
+    exp(sm_scale * q[t, g] . k[i, h] - lse[t, g]), place i being row i % block_tokens of the i //
+    block_tokens-th selected block. ``query`` [query_heads, head_dim] (a decode step) or
+    [queries, query_heads, head_dim] (a prompt's last queries), FP32, FP16, BF16 or FP64; a place
+    counts for query t when its row lies before the block's valid count and i < ``visible``[t] (int32
+    [queries]; None: all). ``lse`` fp32 [query_heads] or [queries, query_heads]: as ``decode``
+    returned it for these queries, or None to compute it (a first pass over the keys). ``out`` may be
+    ``previous``. The returned lse is -inf for a query that sees nothing; it adds nothing."""
+    device = _cuda_device("attention_weights", query)
+    dtype = _QUERY_DTYPES.get(query.dtype)
+    if dtype is None:
+        raise ValueError(f"unsupported query dtype {query.dtype}")
+    if query.ndim not in (2, 3):
+        raise ValueError("query must be [query_heads, head_dim] or [queries, query_heads, head_dim]")
+    if not query.is_contiguous():
+        query = query.contiguous()
+    n_pool, bt, kvh, d = _check_pool(packed_k, None, scales_k, None, valid_tokens, bits, group_size,
+                                     device)
+    rows = query.shape[:-1]
+    queries = rows[0] if query.ndim == 3 else 1
+    qh = rows[-1]
+    if query.shape[-1] != d:
+        raise ValueError("packed dimension does not match query head dimension")
+    if queries < 1 or qh < 1 or qh % kvh:
+        raise ValueError("query heads must be divisible by KV heads")
+    n_sel = _check_table(block_table, n_pool, device)
+    places = n_sel * bt
+    if visible is not None:
+        _require_cuda("visible", visible, device, torch.int32)
+        if visible.shape != (queries,):
+            raise ValueError("visible must hold one count per query")
+    if previous is not None:
+        _require_stats("previous", previous, kvh, places, torch.float32, device)
+    if out is None:
+        out = torch.empty((kvh, places), dtype=torch.float32, device=device)
+    else:
+        _require_stats("out", out, kvh, places, torch.float32, device)
+    scratch, scratch_bytes, given = None, 0, lse is not None
+    if given:
+        _require_cuda("lse", lse, device, torch.float32)
+        if lse.shape != rows:
+            raise ValueError(f"lse must be {tuple(rows)}, got {tuple(lse.shape)}")
+    else:
+        need = ctypes.c_size_t()
+        _call(device, "kvssd_b200_attention_weights_scratch_size", queries, n_sel, bt, qh, kvh, d,
+              bits, group_size, ctypes.byref(need))
+        scratch_bytes = need.value
+        scratch = torch.empty(scratch_bytes, dtype=torch.uint8, device=device)
+        lse = torch.empty(rows, dtype=torch.float32, device=device)
+    stream = _stream_handle(device)
+    _call(device, "kvssd_b200_attention_weights", query.data_ptr(), dtype, queries,
+          packed_k.data_ptr(), scales_k.data_ptr(), valid_tokens.data_ptr(), _ptr(block_table),
+          _ptr(visible), n_pool, n_sel, bt, qh, kvh, d, bits, group_size, sm_scale, given,
+          lse.data_ptr(), _ptr(previous), 0 if previous is None else previous.stride(0),
+          out.data_ptr(), out.stride(0), _ptr(scratch), scratch_bytes, _status_word(device, stream),
+          stream)
+    return out, lse
+
+
+def evict(weights: torch.Tensor, positions: torch.Tensor, n_tokens: int, keep: int,
+          packed_k: torch.Tensor, packed_v: torch.Tensor, scales_k: torch.Tensor,
+          scales_v: torch.Tensor, valid_tokens: torch.Tensor, *,
+          block_table: torch.Tensor | None = None, sink: int = 0, recent: int = 0,
+          next_position: int | None = None,
+          shared: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    """Compacts a cache of ``n_tokens`` tokens in place to the ``keep`` tokens of the largest
+    accumulated weight; returns (weights, positions) of the compacted cache, shaped as given, 0 and -1
+    from ``keep`` on.
+
+    Place i of the cache is row i % block_tokens of the i // block_tokens-th selected block
+    (``block_table`` entries must differ; None: the pool in order); its blocks before the last hold
+    block_tokens tokens each. ``weights`` fp32 and ``positions`` int32 [kv_heads, places] say what
+    each place has gathered (``attention_weights``) and which token it holds. Each KV head chooses for
+    itself, or all heads together by the sum of their weights when ``shared`` (positions of head 0).
+    Tokens at positions below ``sink`` or among the ``recent`` ones before ``next_position`` (None:
+    n_tokens) are kept in any case; equal weights go by the lower place, a NaN ranks last. The j-th
+    place below ``keep`` that is given up receives the j-th kept token from behind ``keep`` (packed
+    rows, scales, weight, position); the rows from ``keep`` on stay as they were, and
+    ``valid_tokens`` of the selected blocks becomes the rows they still hold."""
+    device = _cuda_device("evict", weights)
+    for name, t, dt in (("packed_k", packed_k, torch.uint8), ("packed_v", packed_v, torch.uint8),
+                        ("scales_k", scales_k, torch.float16),
+                        ("scales_v", scales_v, torch.float16),
+                        ("valid_tokens", valid_tokens, torch.int32)):
+        _require_cuda(name, t, device, dt)
+    if packed_k.ndim != 4 or packed_v.shape != packed_k.shape:
+        raise ValueError("packed KV must match [blocks,tokens,kv_heads,packed_dim]")
+    n_pool, bt, kvh, pd = packed_k.shape
+    if scales_k.ndim != 4 or scales_k.shape[:3] != packed_k.shape[:3] or scales_v.shape != scales_k.shape:
+        raise ValueError("KV scales must match [blocks,tokens,kv_heads,groups]")
+    if valid_tokens.shape != (n_pool,):
+        raise ValueError("valid_tokens must contain one count per block")
+    _require_stats("weights", weights, kvh, None, torch.float32, device)
+    columns = weights.shape[1]
+    _require_stats("positions", positions, kvh, columns, torch.int32, device)
+    n_sel = _check_table(block_table, n_pool, device)
+    if not 1 <= n_tokens <= min(columns, n_sel * bt):
+        raise ValueError("n_tokens must be positive and lie in the selected blocks and in weights")
+    if not 1 <= keep <= n_tokens:
+        raise ValueError("keep must be 1 to n_tokens")
+    if sink < 0 or recent < 0:
+        raise ValueError("sink and recent counts must be non-negative")
+    if sink + recent > keep:
+        raise ValueError("keep must hold the sink and recent tokens")
+    end = n_tokens if next_position is None else next_position
+    recent_from = end - recent if recent else 1 << 40  # behind every position
+    lists = 1 if shared else kvh
+    new_weights = torch.empty((kvh, columns), dtype=torch.float32, device=device)
+    new_positions = torch.empty((kvh, columns), dtype=torch.int32, device=device)
+    scratch = torch.empty(lists * (n_tokens + 1), dtype=torch.int32, device=device)
+    stream = _stream_handle(device)
+    _call(device, "kvssd_b200_evict", weights.data_ptr(), weights.stride(0), positions.data_ptr(),
+          positions.stride(0), n_tokens, keep, sink, recent_from, shared, new_weights.data_ptr(),
+          new_positions.data_ptr(), columns, packed_k.data_ptr(), packed_v.data_ptr(),
+          scales_k.data_ptr(), scales_v.data_ptr(), valid_tokens.data_ptr(), _ptr(block_table),
+          n_pool, n_sel, bt, kvh, pd, scales_k.shape[3], scratch.data_ptr(), 4 * scratch.numel(),
+          _status_word(device, stream), stream)
+    return new_weights, new_positions
+
+
 def default_sm_scale(head_dim: int) -> float:
     return 1.0 / math.sqrt(head_dim)
