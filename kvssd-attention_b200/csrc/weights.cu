@@ -5,9 +5,11 @@
 // `visible` count on, refused blocks). The log-sum-exps come from the attention that has run, or a
 // first pass over the keys computes them.
 //
-// weights_lse_kernel, weights_combine_kernel, weights_kernel: the form for any shape. A CTA takes
-// one KV head and kPlaces places, a warp one place at a time, the lanes the head's dims.
-#include "cache_ops.cuh"
+// head_dim 64, 96, 128 and 256 with scale groups of whole 16 dims and aligned codes run on the
+// tensor cores (weights_tc.cuh). weights_lse_kernel, weights_combine_kernel and weights_kernel are the
+// form for any other shape: a CTA takes one KV head and kPlaces places, a warp one place at a time,
+// the lanes the head's dims.
+#include "weights_tc.cuh"
 
 namespace kvb {
 namespace {
@@ -156,12 +158,31 @@ __global__ void __launch_bounds__(kThreads) weights_kernel(const WeightsArgs a) 
 
 }  // namespace
 
+using TcLauncher = cudaError_t (*)(const WeightsArgs&, cudaStream_t);
+
+TcLauncher tc_launcher(int d, int group) {
+  if (group % 16) return nullptr;
+  switch (d) {
+    case 64: return launch_weights_tc_64;
+    case 96: return launch_weights_tc_96;
+    case 128: return launch_weights_tc_128;
+    case 256: return launch_weights_tc_256;
+    default: return nullptr;
+  }
+}
+
 size_t weights_scratch_bytes(int queries, int qh, int n_sel, int bt) {
+  // the general form's parts; those of the tensor-core form, at most one per 32 places too
   const long long chunks = (static_cast<long long>(n_sel) * bt + kPlaces - 1) / kPlaces;
-  return static_cast<size_t>(chunks) * queries * qh * 2 * sizeof(float);
+  const long long tiles = static_cast<long long>(n_sel) * ((bt + 31) / 32);
+  const long long parts = chunks > tiles ? chunks : tiles;
+  return static_cast<size_t>(parts) * queries * qh * 2 * sizeof(float);
 }
 
 cudaError_t launch_weights(const WeightsArgs& a, cudaStream_t s) {
+  const TcLauncher tc = tc_launcher(a.d, a.group);
+  if (tc && (reinterpret_cast<uintptr_t>(a.kp) | reinterpret_cast<uintptr_t>(a.ks)) % 16 == 0)
+    return tc(a, s);
   const int chunks = (a.n_sel * a.bt + kPlaces - 1) / kPlaces;
   if (!a.lse_in) {
     cudaError_t e = launch_pdl(weights_lse_kernel, dim3(chunks, a.kvh), kThreads, 0, s, a);

@@ -1,0 +1,8 @@
+// Attention weights on the tensor cores, head_dim 128 (kernels: weights_tc.cuh).
+#include "weights_tc.cuh"
+
+namespace kvb {
+cudaError_t launch_weights_tc_128(const WeightsArgs& a, cudaStream_t s) {
+  return weights_tc::launch<128>(a, s);
+}
+}  // namespace kvb
