@@ -1,5 +1,5 @@
-// Attention weights on the tensor cores, head_dim 64 (kernels: weights_tc.cuh).
-#include "weights_tc.cuh"
+// Attention weights on the tensor cores, head_dim 64 (weights_step.cuh, weights_window.cuh).
+#include "weights_tc_launch.cuh"
 
 namespace kvb {
 cudaError_t launch_weights_tc_64(const WeightsArgs& a, cudaStream_t s) {
