@@ -391,7 +391,8 @@ KVSSD_B200_API int kvssd_b200_rotary(const void* x, int dtype, long long x_token
  * equal ones the row holds a mixture). With `frequencies` (else NULL) the keys are rotated first, as
  * kvssd_b200_rotary does but rounded to FP32 once and not to their type. Codes and scales are those
  * of quantize_tensor (src/kvssd/quant.py:49-65), bit for bit, as KVCacheStore.create stores them
- * (src/kvssd/store.py:50-59); a NaN makes its group's scale NaN. Where `valid_tokens` is not NULL the
+ * (src/kvssd/store.py:50-59); a NaN or an infinity makes
+ * its group's scale NaN or infinite, and the group's codes are unspecified. Where `valid_tokens` is not NULL the
  * counts of the written blocks are raised to cover the written rows. key_values and value_values
  * (both or neither NULL) receive the FP16 values that the cache now holds for the tokens,
  * [tokens, kv_heads, head_dim] (dequantize_tensor, src/kvssd/quant.py:68-73), skipped tokens

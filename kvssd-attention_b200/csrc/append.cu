@@ -9,8 +9,8 @@
 // depend on the order of roundings; they are not rounded to the input's type in between.
 //
 // Bound by HBM: the inputs are read once, codes and scales (and, when asked for, the FP16 values
-// that the codes stand for) are written once; the arithmetic of the rotated keys comes close to that
-// time, so it is kept short where it can be (rotate_once, quantize8).
+// that the codes stand for) are written once; the arithmetic comes close to that time, so it works on
+// two elements an instruction and divides by remainders.
 //
 // append_rows_kernel: scale groups and pairs of whole 8 elements, rows on 16 bytes. append_kernel is
 // the form for any other shape and alignment: a CTA takes one token, a warp one scale group after the
@@ -22,10 +22,68 @@ namespace {
 
 constexpr int kThreads = 256;
 
+// Two FP32 numbers in one register pair: one instruction rounds both (PTX add/mul/fma.rn.f32x2).
+struct F2 {
+  unsigned long long v;
+};
+__device__ __forceinline__ F2 f2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ F2 f2(float a) { return f2(a, a); }
+__device__ __forceinline__ float2 parts(F2 x) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x.v));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+// a - b: the product with -1 is exact.
+__device__ __forceinline__ F2 sub2(F2 a, F2 b) { return fma2(b, f2(-1.f), a); }
+
 // (hi, lo) pairs of m cos t and m sin t.
-struct Turn {
+struct alignas(16) Turn {
   float ch, cl, sh, sl;
 };
+
+// sin and cos of f turns, |f| <= 1/2, to 2^-44: the Taylor series on an eighth of a turn to either side
+// of the nearest quarter (the first terms left out: x^15 / 15! and x^16 / 16! at pi / 4).
+__device__ __forceinline__ void sin_cos(double f, double& s, double& c) {
+  const double quarter = rint(4.0 * f);
+  const double x = 6.283185307179586 * fma(-0.25, quarter, f), x2 = x * x;
+  double a = 1.0 / 6227020800.0, b = -1.0 / 87178291200.0;
+  a = fma(a, x2, -1.0 / 39916800.0);
+  b = fma(b, x2, 1.0 / 479001600.0);
+  a = fma(a, x2, 1.0 / 362880.0);
+  b = fma(b, x2, -1.0 / 3628800.0);
+  a = fma(a, x2, -1.0 / 5040.0);
+  b = fma(b, x2, 1.0 / 40320.0);
+  a = fma(a, x2, 1.0 / 120.0);
+  b = fma(b, x2, -1.0 / 720.0);
+  a = fma(a, x2, -1.0 / 6.0);
+  b = fma(b, x2, 1.0 / 24.0);
+  b = fma(b, x2, -0.5);
+  a = fma(a * x2, x, x);
+  b = fma(b, x2, 1.0);
+  const int q = static_cast<int>(quarter) & 3;
+  const double sin0 = q & 1 ? b : a, cos0 = q & 1 ? a : b;
+  s = q & 2 ? -sin0 : sin0;
+  c = (q + 1) & 2 ? -cos0 : cos0;
+}
 
 // A 16-bit element times ch must be exact in FP32 for rotate_once: ch then has 13 bits.
 template <typename T>
@@ -37,7 +95,7 @@ __device__ __forceinline__ float high_part(double x) {
 template <typename T>
 __device__ __forceinline__ Turn make_turn(long long position, double freq, float magnitude) {
   double s, c;
-  sincospi(2.0 * turn_fraction(position, freq), &s, &c);
+  sin_cos(turn_fraction(position, freq), s, c);
   c *= static_cast<double>(magnitude);
   s *= static_cast<double>(magnitude);
   Turn t;
@@ -48,20 +106,19 @@ __device__ __forceinline__ Turn make_turn(long long position, double freq, float
   return t;
 }
 
-// x c + y s rounded once: the rounding errors of the products (none for a 16-bit element, 11 or 8 bits
-// times 13) and of their sum (Knuth's, 6 operations) are added up with the low parts of c and s before
-// the last rounding: 2^-37 of the larger product is what is lost before it.
+// x c + y s rounded once, for two elements: the rounding errors of the products (none for a 16-bit
+// element, 11 or 8 bits times 13) and of their sum (Knuth's, 6 operations) are added up with the low
+// parts of c and s before the last rounding: 2^-37 of the larger product is what is lost before it.
 template <typename T>
-__device__ __forceinline__ float rotate_once(float x, float y, const Turn& t, float sign) {
-  const float sh = sign * t.sh, sl = sign * t.sl;
-  const float p = __fmul_rn(x, t.ch), q = __fmul_rn(y, sh);
-  const float sum = __fadd_rn(p, q);
-  const float b = __fsub_rn(sum, p);
-  float low = __fadd_rn(__fsub_rn(p, __fsub_rn(sum, b)), __fsub_rn(q, b));
+__device__ __forceinline__ F2 rotate_once(F2 x, F2 y, F2 ch, F2 cl, F2 sh, F2 sl) {
+  const F2 p = mul2(x, ch), q = mul2(y, sh);
+  const F2 sum = add2(p, q);
+  const F2 b = sub2(sum, p);
+  F2 low = add2(sub2(p, sub2(sum, b)), sub2(q, b));
   if constexpr (sizeof(T) == 4)
-    low = __fadd_rn(low, __fadd_rn(__fmaf_rn(x, t.ch, -p), __fmaf_rn(y, sh, -q)));
-  low = __fmaf_rn(x, t.cl, __fmaf_rn(y, sl, low));
-  return __fadd_rn(sum, low);
+    low = add2(low, add2(fma2(x, ch, mul2(p, f2(-1.f))), fma2(y, sh, mul2(q, f2(-1.f)))));
+  low = fma2(x, cl, fma2(y, sl, low));
+  return add2(sum, low);
 }
 
 // max that keeps a NaN, so that a group with a NaN gets a NaN scale.
@@ -110,7 +167,10 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a) {
       const int pair = a.interleaved ? d >> 1 : (d < pairs ? d : d - pairs);
       const bool second = a.interleaved ? (d & 1) : d >= pairs;
       const int other = a.interleaved ? d ^ 1 : (second ? d - pairs : d + pairs);
-      return rotate_once<T>(own, to_f32(x[other]), turns[pair], second ? 1.f : -1.f);
+      const Turn& t = turns[pair];
+      const float sign = second ? 1.f : -1.f;
+      return parts(rotate_once<T>(f2(own), f2(to_f32(x[other])), f2(t.ch), f2(t.cl), f2(sign * t.sh),
+                                  f2(sign * t.sl))).x;
     };
     float top = 0.f;
     for (int b = lane; b < bytes; b += 32)
@@ -138,44 +198,55 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a) {
   }
 }
 
-// Codes 0 .. 2^bits - 1 (as floats) of 8 elements of one group: round-half-even(x / scale) + mid with
-// the FP32 quotient. x times the scale's reciprocal is within 2e-6 of that quotient, so the rounding
-// can only differ next to a border between two codes; there (and for anything not finite) the
-// elements are divided.
-template <int BITS>
-__device__ __forceinline__ void quantize8(const float (&x)[8], float scale, float (&code)[8]) {
-  constexpr float kMid = static_cast<float>(1 << (BITS - 1)), kRound = 12582912.f;  // 1.5 2^23
-  const float inverse = __frcp_rn(scale);
-  float far = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float y = __fmaf_rn(x[i], inverse, kMid);
-    code[i] = __fsub_rn(__fadd_rn(y, kRound), kRound);
-    far = max_nan(far, fabsf(y - code[i]));
-  }
-  if (!(far < 0.499998f)) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int n = __float2int_rn(__fdiv_rn(x[i], scale));  // NaN: 0
-      code[i] = static_cast<float>(max(-(1 << (BITS - 1)), min((1 << (BITS - 1)) - 1, n))) + kMid;
-    }
-  }
+// 1 / x to half an ulp and a little: one Newton step from the hardware's approximation.
+__device__ __forceinline__ float reciprocal(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return __fmaf_rn(__fmaf_rn(-x, r, 1.f), r, r);
 }
 
-// Codes packed low bits first. Their weighted sum is a whole number below 2^16, exact in FP32.
+// a / b rounded to nearest, given b's reciprocal: two steps of Markstein's (1990) from a * inverse, each
+// adding the remainder (exact in an FMA) times the inverse; the first brings the quotient within an
+// ulp, the second rounds it. Quotients here are 0 or far from FP32's limits.
+__device__ __forceinline__ F2 quotient(F2 a, F2 b, F2 inverse) {
+  const F2 minus = mul2(b, f2(-1.f));
+  F2 q = mul2(a, inverse);
+  q = fma2(fma2(minus, q, a), inverse, q);
+  return fma2(fma2(minus, q, a), inverse, q);
+}
+
+// Quantizes 8 elements of one group: codes 0 .. 2^bits - 1 as floats. Adding 1.5 2^23 + mid rounds the
+// quotient half to even and adds the (even) midpoint.
 template <int BITS>
-__device__ __forceinline__ uint32_t pack8(const float (&code)[8]) {
-  constexpr int kHalf = 16 / BITS;  // codes of 16 bits
-  uint32_t part[8 / kHalf];
+__device__ __forceinline__ void quantize8(const F2 (&x)[4], float scale, F2 (&code)[4]) {
+  constexpr float kRound = 12582912.f;
+  const F2 b = f2(scale), inverse = f2(reciprocal(scale));
 #pragma unroll
-  for (int k = 0; k < 8 / kHalf; ++k) {
-    float sum = code[k * kHalf + kHalf - 1];
-#pragma unroll
-    for (int i = kHalf - 2; i >= 0; --i)
-      sum = __fmaf_rn(sum, static_cast<float>(1 << BITS), code[k * kHalf + i]);
-    part[k] = __float_as_uint(sum + 8388608.f) & 0xFFFFu;
-  }
-  return BITS == 4 ? part[0] | part[8 / kHalf - 1] << 16 : part[0];
+  for (int i = 0; i < 4; ++i)
+    code[i] = add2(add2(quotient(x[i], b, inverse), f2(kRound + (1 << (BITS - 1)))), f2(-kRound));
+}
+
+// max|x| / (2^(bits-1) - 1), at least 1e-8 over that.
+template <int BITS>
+__device__ __forceinline__ float scale_of(float top) {
+  top = max_nan(top, 1e-8f);
+  if constexpr (BITS == 2) return top;
+  const float scale = parts(quotient(f2(top), f2(7.f), f2(1.f / 7.f))).x;
+  return top < INFINITY ? scale : top;  // an infinity or a NaN shows in the scale
+}
+
+// Codes packed low bits first. Weighted sums of codes are whole numbers below 2^16, exact in FP32.
+template <int BITS>
+__device__ __forceinline__ uint32_t pack8(const F2 (&code)[4]) {
+  // even codes in one half, odd ones in the other
+  constexpr float kStep = static_cast<float>(1 << (2 * BITS)), kOdd = static_cast<float>(1 << BITS);
+  const auto word = [&](F2 sum) {
+    const float2 two = parts(sum);
+    return __float_as_uint(__fmaf_rn(two.y, kOdd, two.x) + 8388608.f) & 0xFFFFu;
+  };
+  const F2 low = fma2(code[1], f2(kStep), code[0]), high = fma2(code[3], f2(kStep), code[2]);
+  if constexpr (BITS == 4) return word(low) | word(high) << 16;
+  return word(fma2(high, f2(kStep * kStep), low));
 }
 
 // Eight elements of a lane, as loaded.
@@ -188,16 +259,17 @@ struct alignas(16) Eight {
 // a time; a task is kIters such steps over the heads of one token's keys or values, their loads all in
 // flight at once. The cos and sin of the token's pairs are computed by the task's lanes and handed
 // around through shared memory, then stay in registers over the heads; a rotation's other element comes
-// from a lane of the same row (half layout) or is the lane's own (interleaved).
-template <typename T, int BITS, bool INTERLEAVED, int kIters>
-__global__ void __launch_bounds__(kThreads) append_rows_kernel(const AppendArgs a, int chunks) {
+// from a lane of the same row (half layout) or is the lane's own (interleaved). kGroupLanes: the lanes
+// of a scale group, 0: any number of them.
+template <typename T, int BITS, bool INTERLEAVED, int kIters, int kGroupLanes>
+__global__ void __launch_bounds__(kThreads, kIters == 4 && sizeof(T) == 2 ? 3 : 2) append_rows_kernel(const AppendArgs a, int chunks, unsigned per_lane) {
   extern __shared__ Turn turns[];  // [warps][pairs]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int lanes = a.d / 8, rows = 32 / lanes;  // lanes of a row, rows of a warp
-  const int l = lane % lanes, row = lane / lanes;
-  const int task = blockIdx.x * (kThreads / 32) + warp;
-  const int per_token = 2 * chunks;
-  const int token = task / per_token, kv = task % per_token / chunks, chunk = task % chunks;
+  const int lanes = a.d >> 3;                                   // of a row
+  const int rows = 32u * per_lane >> 16, row = lane * per_lane >> 16;  // of a warp; this lane's
+  const int l = lane - row * lanes;
+  const int kv = static_cast<int>(blockIdx.y) >= chunks, chunk = blockIdx.y - kv * chunks;
+  const int token = blockIdx.x * (kThreads / 32) + warp;
   const int pairs = a.freq ? a.pairs : 0;
   pdl_wait();
   pdl_launch();
@@ -213,92 +285,117 @@ __global__ void __launch_bounds__(kThreads) append_rows_kernel(const AppendArgs 
     if (row < rows && h < a.kvh) data[i] = *reinterpret_cast<const Eight<T>*>(x + h * in.head);
   }
   const long long slot = pool_row(a, index_at(a.slots, token));
-  if (kv == 0 && chunk == 0 && lane == 0 && slot >= 0 && a.valid)
-    atomicMax(a.valid + slot / a.bt, static_cast<int>(slot % a.bt) + 1);
+  if (blockIdx.y == 0 && lane == 0 && slot >= 0 && a.valid) {
+    // below 2^32 rows (nearly always) the division is the short one
+    const long long block = slot >> 32 ? slot / a.bt : static_cast<unsigned>(slot) / static_cast<unsigned>(a.bt);
+    atomicMax(a.valid + block, static_cast<int>(slot - block * a.bt) + 1);
+  }
 
-  // the turns of this lane's elements; none for a value, or an element behind the rotated part
-  constexpr int kTurns = INTERLEAVED ? 4 : 8;
-  Turn turn[kTurns];
-  float sign = 0.f;   // of the other element's sine: half layout
-  int other = lane;   // the lane that holds it
+  // the turns of this lane's elements, in pairs of elements, signs included; no turn for an element
+  // behind the rotated part
+  F2 ch[4], cl[4], sh[4], sl[4];
+  int other = lane;  // the lane that holds the pairs' other elements: half layout
   const bool turning = kv == 0 && pairs > 0;  // the same for the whole warp
   if (turning) {
     Turn* mine = turns + warp * pairs;
     const long long position = index_at(a.positions, token);
-    for (int i = lane; i < pairs; i += 32) mine[i] = make_turn<T>(position, a.freq[i], a.magnitude);
+    // pair i at (i % kRun) * (pairs / kRun) + i / kRun: lanes read consecutive entries
+    constexpr int kRun = INTERLEAVED ? 4 : 8;
+    const int step = pairs / kRun;
+    for (int i = lane; i < pairs; i += 32)
+      mine[i % kRun * step + i / kRun] = make_turn<T>(position, a.freq[i], a.magnitude);
     __syncwarp();
     const bool rotated = row < rows && l * 8 < 2 * pairs, second = l * 8 >= pairs;
-    const int first = INTERLEAVED ? l * 4 : (second ? l * 8 - pairs : l * 8);
+    const Turn* own = mine + (INTERLEAVED || !second ? l : l - pairs / 8);
+    const float sign = second ? 1.f : -1.f;
 #pragma unroll
-    for (int i = 0; i < kTurns; ++i) {
-      turn[i] = {1.f, 0.f, 0.f, 0.f};
-      if (rotated) turn[i] = mine[first + i];
+    for (int i = 0; i < 4; ++i) {
+      ch[i] = f2(1.f), cl[i] = sh[i] = sl[i] = f2(0.f);
+      if (!rotated) continue;
+      if constexpr (INTERLEAVED) {
+        const Turn t = own[i * step];
+        ch[i] = f2(t.ch), cl[i] = f2(t.cl), sh[i] = f2(-t.sh, t.sh), sl[i] = f2(-t.sl, t.sl);
+      } else {
+        const Turn t = own[2 * i * step], u = own[(2 * i + 1) * step];
+        ch[i] = f2(t.ch, u.ch), cl[i] = f2(t.cl, u.cl);
+        sh[i] = f2(sign * t.sh, sign * u.sh), sl[i] = f2(sign * t.sl, sign * u.sl);
+      }
     }
-    if (rotated && !INTERLEAVED) {
-      other = second ? lane - pairs / 8 : lane + pairs / 8;
-      sign = second ? 1.f : -1.f;
-    }
+    if (rotated && !INTERLEAVED) other = second ? lane - pairs / 8 : lane + pairs / 8;
   }
-  const int group_lanes = a.group / 8, groups = a.d / a.group;
-  const bool butterfly = (group_lanes & (group_lanes - 1)) == 0;
+  const int group_lanes = kGroupLanes ? kGroupLanes : a.group / 8, groups = a.d / a.group;
   constexpr float kMid = static_cast<float>(1 << (BITS - 1));
+  // this lane's outputs of its first head; those of the next are rows heads on
+  const long long at = slot * a.kvh + head0;
+  uint8_t* codes = a.packed[kv] + at * (lanes * BITS) + l * BITS;
+  __half* scales = a.scales[kv] + at * groups + l / group_lanes;
+  const bool leads = l == l / group_lanes * group_lanes;
+  __half* values = a.values[kv];
+  if (values) values += ((static_cast<long long>(token) * a.kvh + head0) * lanes + l) * 8;
 #pragma unroll
   for (int i = 0; i < kIters; ++i) {
     const int h = head0 + i * rows;
     if (h - row >= a.kvh) break;  // the same for the whole warp
-    float v[8];
+    F2 v[4];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = to_f32(data[i].e[k]);
+    for (int k = 0; k < 4; ++k) v[k] = f2(to_f32(data[i].e[2 * k]), to_f32(data[i].e[2 * k + 1]));
     if (turning) {
-      float w[8];
-      if constexpr (INTERLEAVED) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) w[k] = rotate_once<T>(v[k], v[k ^ 1], turn[k / 2], k & 1 ? 1.f : -1.f);
-      } else {
-        Eight<T> there;
+      Eight<T> there;
+      if constexpr (!INTERLEAVED) {
         const uint32_t* from = reinterpret_cast<const uint32_t*>(&data[i]);
         uint32_t* to = reinterpret_cast<uint32_t*>(&there);
 #pragma unroll
         for (int k = 0; k < static_cast<int>(sizeof(Eight<T>) / 4); ++k)
           to[k] = __shfl_sync(0xffffffffu, from[k], other);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) w[k] = rotate_once<T>(v[k], to_f32(there.e[k]), turn[k], sign);
       }
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = w[k];
+      for (int k = 0; k < 4; ++k) {
+        F2 w;
+        if constexpr (INTERLEAVED) {
+          const float2 two = parts(v[k]);
+          w = f2(two.y, two.x);
+        } else {
+          w = f2(to_f32(there.e[2 * k]), to_f32(there.e[2 * k + 1]));
+        }
+        v[k] = rotate_once<T>(v[k], w, ch[k], cl[k], sh[k], sl[k]);
+      }
     }
     float top = 0.f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) top = max_nan(top, fabsf(v[k]));
-    if (butterfly) {
-      for (int o = 1; o < group_lanes; o <<= 1)
-        top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+    for (int k = 0; k < 4; ++k) {
+      const float2 two = parts(v[k]);
+      top = max_nan(top, max_nan(fabsf(two.x), fabsf(two.y)));
+    }
+    if constexpr (kGroupLanes > 0) {
+#pragma unroll
+      for (int o = 1; o < kGroupLanes; o <<= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
     } else {
       const int base = row * lanes + l / group_lanes * group_lanes;
-      float all = top;
-      for (int o = 0; o < group_lanes; ++o) all = max_nan(all, __shfl_sync(0xffffffffu, top, base + o));
-      top = all;
+      const float own = top;
+      for (int o = 0; o < group_lanes; ++o) top = max_nan(top, __shfl_sync(0xffffffffu, own, base + o));
     }
-    const float scale = __fdiv_rn(max_nan(top, 1e-8f), kMid - 1.f);
+    const float scale = scale_of<BITS>(top);
     const __half held = __float2half_rn(scale);
-    float code[8];
+    F2 code[4];
     quantize8<BITS>(v, scale, code);
-    if (row >= rows || h >= a.kvh) continue;
-    if (slot >= 0) {
-      const long long at = slot * a.kvh + h;
+    const bool mine = row < rows && h < a.kvh;
+    if (mine && slot >= 0) {
       const uint32_t bytes = pack8<BITS>(code);
-      uint8_t* codes = a.packed[kv] + at * (a.d * BITS / 8) + l * BITS;
-      if constexpr (BITS == 4) *reinterpret_cast<uint32_t*>(codes) = bytes;
-      else *reinterpret_cast<uint16_t*>(codes) = static_cast<uint16_t>(bytes);
-      if (l % group_lanes == 0) a.scales[kv][at * groups + l / group_lanes] = held;
+      uint8_t* to = codes + i * (rows * lanes * BITS);
+      if constexpr (BITS == 4) *reinterpret_cast<uint32_t*>(to) = bytes;
+      else *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(bytes);
+      if (leads) scales[i * (rows * groups)] = held;
     }
-    if (a.values[kv]) {
-      const float unit = __half2float(held);
-      Eight<__half> out;
+    if (mine && values) {
+      const F2 unit = f2(__half2float(held));
+      uint4 out;
+      uint32_t* word = reinterpret_cast<uint32_t*>(&out);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) out.e[k] = __float2half_rn(__fmul_rn(code[k] - kMid, unit));
-      *reinterpret_cast<Eight<__half>*>(a.values[kv] + (static_cast<long long>(token) * a.kvh + h) * a.d +
-                                        l * 8) = out;
+      for (int k = 0; k < 4; ++k) {
+        const float2 two = parts(mul2(add2(code[k], f2(-kMid)), unit));
+        word[k] = h2_as_u32(__floats2half2_rn(two.x, two.y));
+      }
+      *reinterpret_cast<uint4*>(values + i * (rows * lanes * 8)) = out;
     }
   }
 }
@@ -311,12 +408,14 @@ cudaError_t launch_rows(const AppendArgs& a, cudaStream_t s) {
   const int long_chunks = (a.kvh + 4 * rows - 1) / (4 * rows), short_chunks = (a.kvh + rows - 1) / rows;
   const bool few = 2ll * a.tokens * long_chunks < 148 * 16;
   const int chunks = few ? short_chunks : long_chunks;
-  const long long tasks = 2ll * a.tokens * chunks;
-  if (tasks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
   const size_t smem = a.freq ? static_cast<size_t>(warps) * a.pairs * sizeof(Turn) : 0;
-  const auto kernel = few ? append_rows_kernel<T, BITS, INTERLEAVED, 1> : append_rows_kernel<T, BITS, INTERLEAVED, 4>;
-  return launch_pdl(kernel, dim3(static_cast<unsigned>((tasks + warps - 1) / warps)), kThreads, smem, s,
-                    a, chunks);
+  auto kernel = few ? append_rows_kernel<T, BITS, INTERLEAVED, 1, 0> : append_rows_kernel<T, BITS, INTERLEAVED, 4, 0>;
+  if (a.group == 32)
+    kernel = few ? append_rows_kernel<T, BITS, INTERLEAVED, 1, 4> : append_rows_kernel<T, BITS, INTERLEAVED, 4, 4>;
+  // lane / lanes as a product: 2^16 / lanes rounded up is exact for 32 lanes
+  const unsigned per_lane = (65536u + a.d / 8 - 1) / (a.d / 8);
+  return launch_pdl(kernel, dim3((a.tokens + warps - 1) / warps, 2 * chunks), kThreads, smem, s, a, chunks,
+                    per_lane);
 }
 
 // Whether append_rows_kernel takes this call.
