@@ -660,32 +660,44 @@ _ELEMENT_DTYPES = {torch.float32: _native.Q_F32, torch.float16: _native.Q_F16,
 _INDEX_DTYPES = {torch.int32: 0, torch.int64: 1}
 
 
-def _call(device: torch.device, name: str, *args) -> None:
-    """Calls an entry point with ``device`` current."""
-    fn = getattr(_native.library(), name)
-    if torch.cuda.current_device() == device.index:
+# The operators below are called once per layer and step, on tensors that differ in nothing but their
+# contents, and their kernels take a few microseconds: what a call costs on the host is part of what it
+# costs. Each checks its tensors in one expression and looks for the reason only when that fails.
+
+_entry_points: dict[str, object] = {}
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _call(index: int, name: str, *args) -> None:
+    """Calls an entry point with device ``index`` current."""
+    fn = _entry_points.get(name)
+    if fn is None:
+        fn = _entry_points[name] = getattr(_native.library(), name)
+    if torch.cuda.current_device() == index:
         status = fn(*args)
     else:
-        with torch.cuda.device(device):
+        with torch.cuda.device(index):
             status = fn(*args)
     if status:
         _native.check(status, name)
 
 
-def _cuda_device(name: str, t: torch.Tensor) -> torch.device:
-    if t.device.type != "cuda":
+def _device_index(name: str, t: torch.Tensor) -> int:
+    if not t.is_cuda:
         raise RuntimeError(f"{name} requires a CUDA device, got {t.device}")
-    return t.device
+    return t.get_device()
 
 
-def _status_word(device: torch.device, stream: int) -> int | None:
+def _status_word(index: int, stream: int) -> int | None:
     """Address of the stream's sticky status word (read_device_status, status_watch); None during a
     graph capture on a stream that has none yet, since creating it would be captured."""
-    ws = _workspaces._buffers.get((device.index, stream))
+    ws = _workspaces._buffers.get((index, stream))
     if ws is None:
         if torch.cuda.is_current_stream_capturing():
             return None
-        ws = _workspaces.get(device, torch.cuda.current_stream(device), _WORKSPACE_HEADER)
+        ws = _workspaces.get(torch.device("cuda", index), torch.cuda.current_stream(index),
+                             _WORKSPACE_HEADER)
     return ws.data_ptr()
 
 
@@ -726,33 +738,42 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, 
     rotary.RotaryEmbedding for the usual scalings). The first 2 * pairs dims of a head are rotated
     -- pair i is dims (i, i + pairs), or (2i, 2i + 1) when ``interleaved`` --, the dims behind are
     copied. Angles are FP64, products FP32, rounded once."""
-    device = _cuda_device("rotary", x)
+    index = _device_index("rotary", x)
     dtype = _ELEMENT_DTYPES.get(x.dtype)
     if dtype is None:
         raise ValueError(f"unsupported element type {x.dtype}")
     if x.ndim != 3:
         raise ValueError("x must be [tokens, heads, head_dim]")
-    tokens, heads, d = x.shape
-    if x.stride(2) != 1 and out is None:
-        x = x.contiguous()
-    _require_rows("x", x, x.shape, x.dtype, device)
-    kind = _index_kind("positions", positions, tokens, device)
-    pairs = _check_frequencies(frequencies, d, device)
     if out is None:
-        out = torch.empty((tokens, heads, d), dtype=x.dtype, device=device)
+        if x.stride(2) != 1:
+            x = x.contiguous()
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
     else:
-        _require_rows("out", out, x.shape, x.dtype, device)
-        near, far = sorted(((out.stride(0), tokens), (out.stride(1), heads)))
+        _require_rows("x", x, x.shape, x.dtype, x.device)
+        _require_rows("out", out, x.shape, x.dtype, x.device)
+        near, far = sorted(((out.stride(0), x.shape[0]), (out.stride(1), x.shape[1])))
+        d = x.shape[2]
         if (near[1] > 1 and near[0] < d) or (far[1] > 1 and far[0] < max(near[0] * near[1], d)):
             raise ValueError("out must not overlap itself")
-    _call(device, "kvssd_b200_rotary", x.data_ptr(), dtype, x.stride(0), x.stride(1), tokens, heads,
-          d, positions.data_ptr(), kind, frequencies.data_ptr(), pairs, interleaved, magnitude,
-          out.data_ptr(), out.stride(0), out.stride(1), _stream_handle(device))
+    tokens, heads, d = x.shape
+    kind = _INDEX_DTYPES.get(positions.dtype)
+    if (kind is None or positions.shape != (tokens,) or positions.get_device() != index
+            or not positions.is_contiguous()):
+        _index_kind("positions", positions, tokens, x.device)
+    if (frequencies.dtype is not torch.float64 or frequencies.ndim != 1
+            or not 2 <= 2 * frequencies.shape[0] <= d or frequencies.get_device() != index
+            or not frequencies.is_contiguous()):
+        _check_frequencies(frequencies, d, x.device)
+    token, head, _ = x.stride()
+    out_token, out_head, _ = out.stride()
+    _call(index, "kvssd_b200_rotary", x.data_ptr(), dtype, token, head, tokens, heads, d,
+          positions.data_ptr(), kind, frequencies.data_ptr(), frequencies.shape[0], interleaved,
+          magnitude, out.data_ptr(), out_token, out_head, _raw_stream(index))
     return out
 
 
 def _check_pool(packed_k, packed_v, scales_k, scales_v, valid_tokens, bits, group_size, device):
-    """Checks the tensors of a block pool; returns (n_pool, block_tokens, kv_heads, head_dim)."""
+    """Finds what is wrong with the tensors of a block pool, if anything is."""
     for name, t, dt in (("packed_k", packed_k, torch.uint8), ("packed_v", packed_v, torch.uint8),
                         ("scales_k", scales_k, torch.float16),
                         ("scales_v", scales_v, torch.float16),
@@ -772,7 +793,6 @@ def _check_pool(packed_k, packed_v, scales_k, scales_v, valid_tokens, bits, grou
         raise ValueError("KV scales must match [blocks,tokens,kv_heads,groups]")
     if valid_tokens is not None and valid_tokens.shape != (n_pool,):
         raise ValueError("valid_tokens must contain one count per block")
-    return n_pool, bt, kvh, d
 
 
 def append(key: torch.Tensor, value: torch.Tensor, slots: torch.Tensor, packed_k: torch.Tensor,
@@ -792,37 +812,65 @@ def append(key: torch.Tensor, value: torch.Tensor, slots: torch.Tensor, packed_k
     blocks are raised to cover the written rows. ``values=True`` returns the FP16 keys and values that
     the cache now holds for the tokens ([tokens, kv_heads, head_dim], skipped tokens included), for a
     prompt's own attention to see what later decodes will see."""
-    device = _cuda_device("append", key)
+    index = _device_index("append", key)
     dtype = _ELEMENT_DTYPES.get(key.dtype)
     if dtype is None:
         raise ValueError(f"unsupported element type {key.dtype}")
     if key.ndim != 3:
         raise ValueError("key must be [tokens, kv_heads, head_dim]")
-    n_pool, bt, kvh, d = _check_pool(packed_k, packed_v, scales_k, scales_v, valid_tokens, bits,
-                                     group_size, device)
-    tokens = key.shape[0]
-    _require_rows("key", key, (tokens, kvh, d), key.dtype, device)
-    _require_rows("value", value, (tokens, kvh, d), key.dtype, device)
-    slot_kind = _index_kind("slots", slots, tokens, device)
+    pool = packed_k.shape
+    scales = scales_k.shape
+    if (len(pool) != 4 or packed_v.shape != pool or len(scales) != 4 or scales[:3] != pool[:3]
+            or scales_v.shape != scales or bits not in (2, 4) or pool[3] * 8 != scales[3] * group_size * bits
+            or packed_k.dtype is not torch.uint8 or packed_v.dtype is not torch.uint8
+            or scales_k.dtype is not torch.float16 or scales_v.dtype is not torch.float16
+            or packed_k.get_device() != index or packed_v.get_device() != index
+            or scales_k.get_device() != index or scales_v.get_device() != index
+            or not packed_k.is_contiguous() or not packed_v.is_contiguous()
+            or not scales_k.is_contiguous() or not scales_v.is_contiguous()
+            or valid_tokens is not None and (
+                valid_tokens.dtype is not torch.int32 or valid_tokens.shape != pool[:1]
+                or valid_tokens.get_device() != index or not valid_tokens.is_contiguous())):
+        _check_pool(packed_k, packed_v, scales_k, scales_v, valid_tokens, bits, group_size, key.device)
+        raise ValueError("packed dimension does not match the scales")
+    n_pool, bt, kvh, pd = pool
+    tokens, d = key.shape[0], pd * 8 // bits
+    shape = (tokens, kvh, d)
+    if (key.shape != shape or value.shape != shape or value.dtype is not key.dtype
+            or value.get_device() != index or key.stride(2) != 1 or value.stride(2) != 1):
+        _require_rows("key", key, shape, key.dtype, key.device)
+        _require_rows("value", value, shape, key.dtype, key.device)
+    slot_kind = _INDEX_DTYPES.get(slots.dtype)
+    if (slot_kind is None or slots.shape != (tokens,) or slots.get_device() != index
+            or not slots.is_contiguous()):
+        _index_kind("slots", slots, tokens, key.device)
+    pos_ptr = freq_ptr = None
     pos_kind = pairs = 0
     if frequencies is not None:
         if positions is None:
             raise ValueError("rotated keys need positions")
-        pos_kind = _index_kind("positions", positions, tokens, device)
-        pairs = _check_frequencies(frequencies, d, device)
-    held = None
+        pos_kind = _INDEX_DTYPES.get(positions.dtype)
+        if (pos_kind is None or positions.shape != (tokens,) or positions.get_device() != index
+                or not positions.is_contiguous()):
+            _index_kind("positions", positions, tokens, key.device)
+        pairs = frequencies.shape[0] if frequencies.ndim == 1 else 0
+        if (frequencies.dtype is not torch.float64 or not 2 <= 2 * pairs <= d
+                or frequencies.get_device() != index or not frequencies.is_contiguous()):
+            _check_frequencies(frequencies, d, key.device)
+        pos_ptr, freq_ptr = positions.data_ptr(), frequencies.data_ptr()
+    held, key_ptr, value_ptr = None, None, None
     if values:
-        held = (torch.empty((tokens, kvh, d), dtype=torch.float16, device=device),
-                torch.empty((tokens, kvh, d), dtype=torch.float16, device=device))
-    stream = _stream_handle(device)
-    _call(device, "kvssd_b200_append", key.data_ptr(), value.data_ptr(), dtype, key.stride(0),
-          key.stride(1), value.stride(0), value.stride(1), tokens, slots.data_ptr(), slot_kind,
-          None if pairs == 0 else positions.data_ptr(), pos_kind,
-          None if pairs == 0 else frequencies.data_ptr(), pairs, interleaved, magnitude,
-          packed_k.data_ptr(), packed_v.data_ptr(), scales_k.data_ptr(), scales_v.data_ptr(),
-          _ptr(valid_tokens), n_pool, bt, kvh, d, bits, group_size,
-          None if held is None else held[0].data_ptr(),
-          None if held is None else held[1].data_ptr(), _status_word(device, stream), stream)
+        held = tuple(torch.empty_like(key, dtype=torch.float16, memory_format=torch.contiguous_format)
+                     for _ in "kv")
+        key_ptr, value_ptr = held[0].data_ptr(), held[1].data_ptr()
+    stream = _raw_stream(index)
+    k_token, k_head, _ = key.stride()
+    v_token, v_head, _ = value.stride()
+    _call(index, "kvssd_b200_append", key.data_ptr(), value.data_ptr(), dtype, k_token, k_head,
+          v_token, v_head, tokens, slots.data_ptr(), slot_kind, pos_ptr, pos_kind, freq_ptr, pairs,
+          interleaved, magnitude, packed_k.data_ptr(), packed_v.data_ptr(), scales_k.data_ptr(),
+          scales_v.data_ptr(), None if valid_tokens is None else valid_tokens.data_ptr(), n_pool, bt,
+          kvh, d, bits, group_size, key_ptr, value_ptr, _status_word(index, stream), stream)
     return held
 
 
@@ -837,7 +885,7 @@ def _check_table(block_table, n_pool: int, device) -> int:
 
 def _require_stats(name: str, t: torch.Tensor, kvh: int, columns: int | None, dtype, device) -> None:
     """A [kv_heads, columns] tensor with contiguous rows."""
-    if t.device != device or t.dtype != dtype or t.ndim != 2 or t.shape[0] != kvh or (
+    if t.dtype is not dtype or t.ndim != 2 or t.shape[0] != kvh or t.device != device or (
             columns is not None and t.shape[1] != columns):
         raise ValueError(f"{name} must be [{kvh}, {columns or 'places'}] {dtype} on {device}, got "
                          f"{tuple(t.shape)} {t.dtype} on {t.device}")
@@ -861,7 +909,7 @@ def attention_weights(query: torch.Tensor, packed_k: torch.Tensor, scales_k: tor
     [queries]; None: all). ``lse`` fp32 [query_heads] or [queries, query_heads]: as ``decode``
     returned it for these queries, or None to compute it (a first pass over the keys). ``out`` may be
     ``previous``. The returned lse is -inf for a query that sees nothing; it adds nothing."""
-    device = _cuda_device("attention_weights", query)
+    index = _device_index("attention_weights", query)
     dtype = _QUERY_DTYPES.get(query.dtype)
     if dtype is None:
         raise ValueError(f"unsupported query dtype {query.dtype}")
@@ -869,8 +917,19 @@ def attention_weights(query: torch.Tensor, packed_k: torch.Tensor, scales_k: tor
         raise ValueError("query must be [query_heads, head_dim] or [queries, query_heads, head_dim]")
     if not query.is_contiguous():
         query = query.contiguous()
-    n_pool, bt, kvh, d = _check_pool(packed_k, None, scales_k, None, valid_tokens, bits, group_size,
-                                     device)
+    pool = packed_k.shape
+    scales = scales_k.shape
+    if (len(pool) != 4 or len(scales) != 4 or scales[:3] != pool[:3] or bits not in (2, 4)
+            or pool[3] * 8 != scales[3] * group_size * bits or packed_k.dtype is not torch.uint8
+            or scales_k.dtype is not torch.float16 or valid_tokens.dtype is not torch.int32
+            or valid_tokens.shape != pool[:1] or packed_k.get_device() != index
+            or scales_k.get_device() != index or valid_tokens.get_device() != index
+            or not packed_k.is_contiguous() or not scales_k.is_contiguous()
+            or not valid_tokens.is_contiguous()):
+        _check_pool(packed_k, None, scales_k, None, valid_tokens, bits, group_size, query.device)
+        raise ValueError("packed dimension does not match the scales")
+    n_pool, bt, kvh, pd = pool
+    d = pd * 8 // bits
     rows = query.shape[:-1]
     queries = rows[0] if query.ndim == 3 else 1
     qh = rows[-1]
@@ -878,37 +937,46 @@ def attention_weights(query: torch.Tensor, packed_k: torch.Tensor, scales_k: tor
         raise ValueError("packed dimension does not match query head dimension")
     if queries < 1 or qh < 1 or qh % kvh:
         raise ValueError("query heads must be divisible by KV heads")
-    n_sel = _check_table(block_table, n_pool, device)
+    table = None
+    n_sel = n_pool
+    if block_table is not None:
+        n_sel = _check_table(block_table, n_pool, query.device)
+        table = block_table.data_ptr()
     places = n_sel * bt
+    seen = None
     if visible is not None:
-        _require_cuda("visible", visible, device, torch.int32)
+        _require_cuda("visible", visible, query.device, torch.int32)
         if visible.shape != (queries,):
             raise ValueError("visible must hold one count per query")
+        seen = visible.data_ptr()
+    before, before_stride = None, 0
     if previous is not None:
-        _require_stats("previous", previous, kvh, places, torch.float32, device)
+        _require_stats("previous", previous, kvh, places, torch.float32, query.device)
+        before, before_stride = previous.data_ptr(), previous.stride(0)
     if out is None:
-        out = torch.empty((kvh, places), dtype=torch.float32, device=device)
+        out = torch.empty((kvh, places), dtype=torch.float32, device=query.device)
     else:
-        _require_stats("out", out, kvh, places, torch.float32, device)
-    scratch, scratch_bytes, given = None, 0, lse is not None
+        _require_stats("out", out, kvh, places, torch.float32, query.device)
+    scratch, scratch_ptr, scratch_bytes, given = None, None, 0, lse is not None
     if given:
-        _require_cuda("lse", lse, device, torch.float32)
-        if lse.shape != rows:
+        if (lse.dtype is not torch.float32 or lse.shape != rows or lse.get_device() != index
+                or not lse.is_contiguous()):
+            _require_cuda("lse", lse, query.device, torch.float32)
             raise ValueError(f"lse must be {tuple(rows)}, got {tuple(lse.shape)}")
     else:
         need = ctypes.c_size_t()
-        _call(device, "kvssd_b200_attention_weights_scratch_size", queries, n_sel, bt, qh, kvh, d,
+        _call(index, "kvssd_b200_attention_weights_scratch_size", queries, n_sel, bt, qh, kvh, d,
               bits, group_size, ctypes.byref(need))
         scratch_bytes = need.value
-        scratch = torch.empty(scratch_bytes, dtype=torch.uint8, device=device)
-        lse = torch.empty(rows, dtype=torch.float32, device=device)
-    stream = _stream_handle(device)
-    _call(device, "kvssd_b200_attention_weights", query.data_ptr(), dtype, queries,
-          packed_k.data_ptr(), scales_k.data_ptr(), valid_tokens.data_ptr(), _ptr(block_table),
-          _ptr(visible), n_pool, n_sel, bt, qh, kvh, d, bits, group_size, sm_scale, given,
-          lse.data_ptr(), _ptr(previous), 0 if previous is None else previous.stride(0),
-          out.data_ptr(), out.stride(0), _ptr(scratch), scratch_bytes, _status_word(device, stream),
-          stream)
+        scratch = torch.empty(scratch_bytes, dtype=torch.uint8, device=query.device)
+        scratch_ptr = scratch.data_ptr()
+        lse = torch.empty(rows, dtype=torch.float32, device=query.device)
+    stream = _raw_stream(index)
+    _call(index, "kvssd_b200_attention_weights", query.data_ptr(), dtype, queries,
+          packed_k.data_ptr(), scales_k.data_ptr(), valid_tokens.data_ptr(), table, seen, n_pool,
+          n_sel, bt, qh, kvh, d, bits, group_size, sm_scale, given, lse.data_ptr(), before,
+          before_stride, out.data_ptr(), out.stride(0), scratch_ptr, scratch_bytes,
+          _status_word(index, stream), stream)
     return out, lse
 
 
@@ -932,23 +1000,31 @@ def evict(weights: torch.Tensor, positions: torch.Tensor, n_tokens: int, keep: i
     place below ``keep`` that is given up receives the j-th kept token from behind ``keep`` (packed
     rows, scales, weight, position); the rows from ``keep`` on stay as they were, and
     ``valid_tokens`` of the selected blocks becomes the rows they still hold."""
-    device = _cuda_device("evict", weights)
-    for name, t, dt in (("packed_k", packed_k, torch.uint8), ("packed_v", packed_v, torch.uint8),
-                        ("scales_k", scales_k, torch.float16),
-                        ("scales_v", scales_v, torch.float16),
-                        ("valid_tokens", valid_tokens, torch.int32)):
-        _require_cuda(name, t, device, dt)
-    if packed_k.ndim != 4 or packed_v.shape != packed_k.shape:
-        raise ValueError("packed KV must match [blocks,tokens,kv_heads,packed_dim]")
-    n_pool, bt, kvh, pd = packed_k.shape
-    if scales_k.ndim != 4 or scales_k.shape[:3] != packed_k.shape[:3] or scales_v.shape != scales_k.shape:
-        raise ValueError("KV scales must match [blocks,tokens,kv_heads,groups]")
-    if valid_tokens.shape != (n_pool,):
-        raise ValueError("valid_tokens must contain one count per block")
-    _require_stats("weights", weights, kvh, None, torch.float32, device)
+    index = _device_index("evict", weights)
+    pool = packed_k.shape
+    scales = scales_k.shape
+    if (len(pool) != 4 or packed_v.shape != pool or len(scales) != 4 or scales[:3] != pool[:3]
+            or scales_v.shape != scales or valid_tokens.shape != pool[:1]
+            or packed_k.dtype is not torch.uint8 or packed_v.dtype is not torch.uint8
+            or scales_k.dtype is not torch.float16 or scales_v.dtype is not torch.float16
+            or valid_tokens.dtype is not torch.int32 or valid_tokens.get_device() != index
+            or packed_k.get_device() != index or packed_v.get_device() != index
+            or scales_k.get_device() != index or scales_v.get_device() != index
+            or not packed_k.is_contiguous() or not packed_v.is_contiguous()
+            or not scales_k.is_contiguous() or not scales_v.is_contiguous()
+            or not valid_tokens.is_contiguous()):
+        for name, t, dt in (("packed_k", packed_k, torch.uint8), ("packed_v", packed_v, torch.uint8),
+                            ("scales_k", scales_k, torch.float16),
+                            ("scales_v", scales_v, torch.float16),
+                            ("valid_tokens", valid_tokens, torch.int32)):
+            _require_cuda(name, t, weights.device, dt)
+        raise ValueError("the pool must be [blocks,tokens,kv_heads,packed_dim] codes, "
+                         "[blocks,tokens,kv_heads,groups] scales and one valid count per block")
+    n_pool, bt, kvh, pd = pool
+    _require_stats("weights", weights, kvh, None, torch.float32, weights.device)
     columns = weights.shape[1]
-    _require_stats("positions", positions, kvh, columns, torch.int32, device)
-    n_sel = _check_table(block_table, n_pool, device)
+    _require_stats("positions", positions, kvh, columns, torch.int32, weights.device)
+    n_sel = _check_table(block_table, n_pool, weights.device)
     if not 1 <= n_tokens <= min(columns, n_sel * bt):
         raise ValueError("n_tokens must be positive and lie in the selected blocks and in weights")
     if not 1 <= keep <= n_tokens:
@@ -960,16 +1036,16 @@ def evict(weights: torch.Tensor, positions: torch.Tensor, n_tokens: int, keep: i
     end = n_tokens if next_position is None else next_position
     recent_from = end - recent if recent else 1 << 40  # behind every position
     lists = 1 if shared else kvh
-    new_weights = torch.empty((kvh, columns), dtype=torch.float32, device=device)
-    new_positions = torch.empty((kvh, columns), dtype=torch.int32, device=device)
-    scratch = torch.empty(lists * (n_tokens + 1), dtype=torch.int32, device=device)
-    stream = _stream_handle(device)
-    _call(device, "kvssd_b200_evict", weights.data_ptr(), weights.stride(0), positions.data_ptr(),
+    new_weights = torch.empty((kvh, columns), dtype=torch.float32, device=weights.device)
+    new_positions = torch.empty((kvh, columns), dtype=torch.int32, device=weights.device)
+    scratch = torch.empty(lists * (n_tokens + 1), dtype=torch.int32, device=weights.device)
+    stream = _raw_stream(index)
+    _call(index, "kvssd_b200_evict", weights.data_ptr(), weights.stride(0), positions.data_ptr(),
           positions.stride(0), n_tokens, keep, sink, recent_from, shared, new_weights.data_ptr(),
           new_positions.data_ptr(), columns, packed_k.data_ptr(), packed_v.data_ptr(),
           scales_k.data_ptr(), scales_v.data_ptr(), valid_tokens.data_ptr(), _ptr(block_table),
-          n_pool, n_sel, bt, kvh, pd, scales_k.shape[3], scratch.data_ptr(), 4 * scratch.numel(),
-          _status_word(device, stream), stream)
+          n_pool, n_sel, bt, kvh, pd, scales[3], scratch.data_ptr(), 4 * lists * (n_tokens + 1),
+          _status_word(index, stream), stream)
     return new_weights, new_positions
 
 
