@@ -22,39 +22,6 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// Two FP32 numbers in one register pair: one instruction rounds both (PTX add/mul/fma.rn.f32x2).
-struct F2 {
-  unsigned long long v;
-};
-__device__ __forceinline__ F2 f2(float a, float b) {
-  F2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ F2 f2(float a) { return f2(a, a); }
-__device__ __forceinline__ float2 parts(F2 x) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x.v));
-  return r;
-}
-__device__ __forceinline__ F2 add2(F2 a, F2 b) {
-  F2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
-  F2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-  F2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return r;
-}
-// a - b: the product with -1 is exact.
-__device__ __forceinline__ F2 sub2(F2 a, F2 b) { return fma2(b, f2(-1.f), a); }
-
 // (hi, lo) pairs of m cos t and m sin t.
 struct alignas(16) Turn {
   float ch, cl, sh, sl;
@@ -252,7 +219,13 @@ __device__ __forceinline__ uint32_t pack8(const F2 (&code)[4]) {
 // Eight elements of a lane, as loaded.
 template <typename T>
 struct alignas(16) Eight {
-  T e[8];
+  static constexpr int kWords = 2 * sizeof(T);
+  uint32_t w[kWords];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < kWords; i += 4)
+      *reinterpret_cast<uint4*>(w + i) = reinterpret_cast<const uint4*>(p)[i / 4];
+  }
 };
 
 // A lane holds 8 consecutive elements of a row (head), a row is d / 8 lanes, a warp 32 / (d / 8) rows at
@@ -282,7 +255,7 @@ __global__ void __launch_bounds__(kThreads, kIters == 4 && sizeof(T) == 2 ? 3 : 
 #pragma unroll
   for (int i = 0; i < kIters; ++i) {
     const int h = head0 + i * rows;
-    if (row < rows && h < a.kvh) data[i] = *reinterpret_cast<const Eight<T>*>(x + h * in.head);
+    if (row < rows && h < a.kvh) data[i].load(x + h * in.head);
   }
   const long long slot = pool_row(a, index_at(a.slots, token));
   if (blockIdx.y == 0 && lane == 0 && slot >= 0 && a.valid) {
@@ -338,15 +311,13 @@ __global__ void __launch_bounds__(kThreads, kIters == 4 && sizeof(T) == 2 ? 3 : 
     if (h - row >= a.kvh) break;  // the same for the whole warp
     F2 v[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = f2(to_f32(data[i].e[2 * k]), to_f32(data[i].e[2 * k + 1]));
+    for (int k = 0; k < 4; ++k) v[k] = unpack_pair<T>(data[i].w, k);
     if (turning) {
       Eight<T> there;
       if constexpr (!INTERLEAVED) {
-        const uint32_t* from = reinterpret_cast<const uint32_t*>(&data[i]);
-        uint32_t* to = reinterpret_cast<uint32_t*>(&there);
 #pragma unroll
-        for (int k = 0; k < static_cast<int>(sizeof(Eight<T>) / 4); ++k)
-          to[k] = __shfl_sync(0xffffffffu, from[k], other);
+        for (int k = 0; k < Eight<T>::kWords; ++k)
+          there.w[k] = __shfl_sync(0xffffffffu, data[i].w[k], other);
       }
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -355,7 +326,7 @@ __global__ void __launch_bounds__(kThreads, kIters == 4 && sizeof(T) == 2 ? 3 : 
           const float2 two = parts(v[k]);
           w = f2(two.y, two.x);
         } else {
-          w = f2(to_f32(there.e[2 * k]), to_f32(there.e[2 * k + 1]));
+          w = unpack_pair<T>(there.w, k);
         }
         v[k] = rotate_once<T>(v[k], w, ch[k], cl[k], sh[k], sl[k]);
       }
@@ -388,14 +359,10 @@ __global__ void __launch_bounds__(kThreads, kIters == 4 && sizeof(T) == 2 ? 3 : 
     }
     if (mine && values) {
       const F2 unit = f2(__half2float(held));
-      uint4 out;
-      uint32_t* word = reinterpret_cast<uint32_t*>(&out);
+      uint32_t out[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float2 two = parts(mul2(add2(code[k], f2(-kMid)), unit));
-        word[k] = h2_as_u32(__floats2half2_rn(two.x, two.y));
-      }
-      *reinterpret_cast<uint4*>(values + i * (rows * lanes * 8)) = out;
+      for (int k = 0; k < 4; ++k) pack_pair<__half>(mul2(add2(code[k], f2(-kMid)), unit), out, k);
+      *reinterpret_cast<uint4*>(values + i * (rows * lanes * 8)) = make_uint4(out[0], out[1], out[2], out[3]);
     }
   }
 }

@@ -65,6 +65,9 @@ int kvssd_b200_rotary(const void* x, int dtype, long long x_token_stride, long l
   if (int st = check_rotation(head_dim, positions, frequencies, pairs)) return st;
   if (static_cast<long long>(heads) * head_dim > 0x1000000ll)
     return report(KVSSD_B200_ERR_UNSUPPORTED, "rows of more than 2^24 elements are not supported");
+  for (const long long stride : {x_token_stride, x_head_stride, out_token_stride, out_head_stride})
+    if (stride > 0x7fffffffll || stride < -0x7fffffffll)
+      return report(KVSSD_B200_ERR_UNSUPPORTED, "strides of 2^31 elements or more are not supported");
   RotaryArgs a{{x, x_token_stride, x_head_stride}, out, out_token_stride, out_head_stride, dtype,
                tokens, heads, head_dim, {positions, positions_int64 ? 1 : 0}, frequencies, pairs,
                interleaved ? 1 : 0, magnitude};

@@ -162,4 +162,74 @@ __device__ __forceinline__ double turn_fraction(long long position, double freq)
   return (hi - rint(hi)) + lo;
 }
 
+// Two FP32 numbers in one register pair: one instruction rounds both (PTX add/mul/fma.rn.f32x2).
+struct F2 {
+  unsigned long long v;
+};
+__device__ __forceinline__ F2 f2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ F2 f2(float a) { return f2(a, a); }
+__device__ __forceinline__ float2 parts(F2 x) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x.v));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+// a - b: the product with -1 is exact.
+__device__ __forceinline__ F2 sub2(F2 a, F2 b) { return fma2(b, f2(-1.f), a); }
+
+// Vectors of N elements as 32-bit words: pairs of 16-bit elements are taken apart and put together a word
+// at a time (arrays of 16-bit elements cost a register and several instructions each).
+template <typename T>
+__device__ __forceinline__ F2 unpack_pair(const uint32_t* w, int i);
+template <>
+__device__ __forceinline__ F2 unpack_pair<float>(const uint32_t* w, int i) {
+  return f2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+}
+template <>
+__device__ __forceinline__ F2 unpack_pair<__half>(const uint32_t* w, int i) {
+  const float2 two = __half22float2(u32_as_h2(w[i]));
+  return f2(two.x, two.y);
+}
+template <>
+__device__ __forceinline__ F2 unpack_pair<__nv_bfloat16>(const uint32_t* w, int i) {
+  return f2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
+}
+template <typename T>
+__device__ __forceinline__ void pack_pair(F2 x, uint32_t* w, int i);
+template <>
+__device__ __forceinline__ void pack_pair<float>(F2 x, uint32_t* w, int i) {
+  const float2 two = parts(x);
+  w[2 * i] = __float_as_uint(two.x);
+  w[2 * i + 1] = __float_as_uint(two.y);
+}
+template <>
+__device__ __forceinline__ void pack_pair<__half>(F2 x, uint32_t* w, int i) {
+  const float2 two = parts(x);
+  w[i] = h2_as_u32(__floats2half2_rn(two.x, two.y));
+}
+template <>
+__device__ __forceinline__ void pack_pair<__nv_bfloat16>(F2 x, uint32_t* w, int i) {
+  const float2 two = parts(x);
+  const __nv_bfloat162 b = __floats2bfloat162_rn(two.x, two.y);
+  memcpy(w + i, &b, 4);
+}
+
 }  // namespace kvb
