@@ -256,6 +256,7 @@ __global__ void __launch_bounds__(kThreads, kIters == 4 && sizeof(T) == 2 ? 3 : 
   for (int i = 0; i < kIters; ++i) {
     const int h = head0 + i * rows;
     if (row < rows && h < a.kvh) data[i].load(x + h * in.head);
+    else data[i] = {};
   }
   const long long slot = pool_row(a, index_at(a.slots, token));
   if (blockIdx.y == 0 && lane == 0 && slot >= 0 && a.valid) {
@@ -307,8 +308,8 @@ __global__ void __launch_bounds__(kThreads, kIters == 4 && sizeof(T) == 2 ? 3 : 
   if (values) values += ((static_cast<long long>(token) * a.kvh + head0) * lanes + l) * 8;
 #pragma unroll
   for (int i = 0; i < kIters; ++i) {
-    const int h = head0 + i * rows;
-    if (h - row >= a.kvh) break;  // the same for the whole warp
+    // no early end: the iterations' chains of dependent operations overlap
+    const bool mine = row < rows && head0 + i * rows < a.kvh;
     F2 v[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) v[k] = unpack_pair<T>(data[i].w, k);
@@ -349,14 +350,13 @@ __global__ void __launch_bounds__(kThreads, kIters == 4 && sizeof(T) == 2 ? 3 : 
     const __half held = __float2half_rn(scale);
     F2 code[4];
     quantize8<BITS>(v, scale, code);
-    const bool mine = row < rows && h < a.kvh;
+    const uint32_t bytes = pack8<BITS>(code);
+    uint8_t* to = codes + i * (rows * lanes * BITS);
     if (mine && slot >= 0) {
-      const uint32_t bytes = pack8<BITS>(code);
-      uint8_t* to = codes + i * (rows * lanes * BITS);
       if constexpr (BITS == 4) *reinterpret_cast<uint32_t*>(to) = bytes;
       else *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(bytes);
-      if (leads) scales[i * (rows * groups)] = held;
     }
+    if (mine && slot >= 0 && leads) scales[i * (rows * groups)] = held;
     if (mine && values) {
       const F2 unit = f2(__half2float(held));
       uint32_t out[4];

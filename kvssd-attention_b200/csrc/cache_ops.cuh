@@ -126,6 +126,19 @@ cudaError_t launch_pdl(void (*kernel)(Params...), dim3 grid, int threads, size_t
   return cudaLaunchKernelEx(&cfg, kernel, Params(args)...);
 }
 
+// n / d for 0 <= n < 2^31 as a product and a shift (Granlund and Montgomery, 1994).
+struct Divisor {
+  unsigned factor, shift;
+};
+inline Divisor divisor(unsigned d) {
+  unsigned shift = 0;
+  while ((1ull << shift) < d) ++shift;
+  return {static_cast<unsigned>((((1ull << shift) - d) << 32) / d + 1), shift};
+}
+__device__ __forceinline__ int divide(int n, Divisor d) {
+  return static_cast<int>((__umulhi(static_cast<unsigned>(n), d.factor) + static_cast<unsigned>(n)) >> d.shift);
+}
+
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_launch() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");

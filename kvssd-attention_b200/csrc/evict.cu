@@ -483,19 +483,6 @@ __global__ void __launch_bounds__(kThreads) evict_select_kernel(const EvictArgs 
   cluster_wait();
 }
 
-// n / d for 0 <= n < 2^31 as a product and a shift (Granlund and Montgomery, 1994).
-struct Divisor {
-  unsigned factor, shift;
-};
-Divisor divisor(unsigned d) {
-  unsigned shift = 0;
-  while ((1ull << shift) < d) ++shift;
-  return {static_cast<unsigned>((((1ull << shift) - d) << 32) / d + 1), shift};
-}
-__device__ __forceinline__ int divide(int n, Divisor d) {
-  return static_cast<int>((__umulhi(static_cast<unsigned>(n), d.factor) + static_cast<unsigned>(n)) >> d.shift);
-}
-
 // Pool row (in tokens) of a place, or -1 for a refused block.
 __device__ __forceinline__ long long token_row(const EvictArgs& a, int place, Divisor bt) {
   const int slot = divide(place, bt);

@@ -279,12 +279,16 @@ def check_weights(query, kp, ks, valid, bits, group, scale, *, lse=None, table=N
     prev = 0.0 if previous is None else previous.double().cpu().numpy()
     tol = w * (np.expm1(2 * off) + 2.0**-18) + (np.abs(prev) + w) * 2.0**-23 + 1e-37
     out, out_lse = got
-    d = np.abs(out.double().cpu().numpy() - (w + prev))
-    assert (d <= tol).all(), (d - tol).max()
+    mine = out.double().cpu().numpy()
+    d = np.abs(mine - (w + prev))
+    broken = np.isnan(w)  # an infinite scale times a zero code: the kernel says so too
+    assert np.array_equal(np.isnan(mine), broken)
+    assert (d <= tol)[~broken].all(), (d - tol)[~broken].max()
     if lse is None:
         l = out_lse.double().cpu().numpy().reshape(full.shape)
         assert np.array_equal(l == -np.inf, full == -np.inf)
-        live = full != -np.inf
+        assert np.array_equal(np.isnan(l), np.isnan(full))
+        live = np.isfinite(full)
         assert (np.abs(l - full)[live] <= off.max() + 2.0**-20 + 2.0**-23 * np.abs(full[live])).all()
 
 
@@ -323,7 +327,65 @@ def test_weights(case, name):
     check_weights(query, kp, ks, valid, bits, group, scale, table=table, lse=lse, got=given)
 
 
-@pytest.mark.parametrize("geometry", [(4, 32, 8, 4, 128, 4, 32), (4, 20, 2, 3, 96, 4, 48)])
+WINDOWS = [  # nb, bt, kvh, gqa, d, bits, group, queries
+    (3, 128, 2, 4, 128, 4, 32, 32), (3, 128, 2, 4, 128, 2, 32, 32), (7, 40, 1, 12, 64, 4, 64, 5),
+    (5, 100, 3, 1, 96, 4, 32, 50), (5, 100, 2, 2, 96, 2, 96, 33), (9, 64, 2, 8, 128, 4, 128, 40),
+    (40, 17, 1, 3, 64, 2, 32, 64), (1, 1, 1, 33, 128, 4, 32, 1), (2, 300, 1, 129, 64, 4, 32, 2)]
+
+
+@pytest.mark.parametrize("name", ["f32", "f16", "bf16", "f64"])
+@pytest.mark.parametrize("case", WINDOWS)
+def test_weights_windows(case, name):
+    """More than 32 query rows a KV head: causal, padded, with given and computed log-sum-exps."""
+    nb, bt, kvh, gqa, d, bits, group, queries = case
+    g = gen(sum(case))
+    kp, ks = key_pool(nb, bt, kvh, d, bits, group, 6, outliers=bits == 2)
+    query = (torch.randn(queries, kvh * gqa, d, generator=g) * 1.3).to(
+        {**TYPES, "f64": torch.float64}[name]).to(DEV)
+    n = nb * bt - bt // 3
+    valid = torch.full((nb,), bt, dtype=torch.int32)
+    valid[-1] = bt - bt // 3
+    valid = valid.to(DEV)
+    visible = (n - queries + 1 + torch.arange(queries)).int()
+    visible[queries // 2] = 0
+    visible = visible.to(DEV)
+    previous = torch.rand(kvh, nb * bt, generator=g).to(DEV)
+    table = torch.randint(0, nb, (nb + 1,), generator=g).int().to(DEV)
+    scale = 1 / math.sqrt(d)
+    got = ops.attention_weights(query, kp, ks, valid, bits, group, scale)
+    check_weights(query, kp, ks, valid, bits, group, scale, got=got)
+    got = ops.attention_weights(query, kp, ks, valid, bits, group, -scale, visible=visible, previous=previous)
+    check_weights(query, kp, ks, valid, bits, group, -scale, visible=visible, previous=previous, got=got)
+    lse = got[1] + 0.25
+    given = ops.attention_weights(query, kp, ks, valid, bits, group, scale, block_table=table, lse=lse)
+    check_weights(query, kp, ks, valid, bits, group, scale, table=table, lse=lse, got=given)
+    zero = ops.attention_weights(query, kp, ks, valid, bits, group, 0.0, visible=visible)
+    check_weights(query, kp, ks, valid, bits, group, 0.0, visible=visible, got=zero)
+
+
+@pytest.mark.parametrize("bits", [2, 4])
+@pytest.mark.parametrize("queries", [1, 16])
+def test_weights_scales_at_the_end_of_fp16(bits, queries):
+    """Key scales up to FP16's largest number (code times scale leaves FP16's range) and down to its
+    smallest, in different tiles and beside each other; the scale brings the scores back to size. In
+    FP16 the largest ones round to infinity: those keys' scores are not numbers, here and there."""
+    kp, ks = key_pool(6, 128, 2, 128, bits, 32, 4)
+    ks[0] *= 65504 / ks[0].max()
+    ks[1, ::2] *= 30000 / ks[1].max()
+    ks[2] = 2.0**-24
+    ks[3, 5:9] = 6e-8
+    valid = torch.full((6,), 128, dtype=torch.int32, device=DEV)
+    query = torch.randn(queries, 8, 128, generator=gen(6)).to(DEV)
+    for finite in (False, True):
+        if finite:
+            ks.clamp_(max=65504)
+        for t, scale in ((torch.float32, 1e-6), (torch.float16, 2e-6)):
+            got = ops.attention_weights(query.to(t), kp, ks, valid, bits, 32, scale)
+            check_weights(query.to(t), kp, ks, valid, bits, 32, scale, got=got)
+
+
+@pytest.mark.parametrize("geometry", [(4, 32, 8, 4, 128, 4, 32), (4, 20, 2, 3, 96, 4, 48),
+                                      (3, 100, 2, 12, 128, 4, 32), (3, 100, 2, 12, 64, 2, 32)])
 def test_weights_masks_and_odd_values(geometry):
     nb, bt, kvh, gqa, d, bits, group = geometry
     kp, ks = key_pool(nb, bt, kvh, d, bits, group, 9)
