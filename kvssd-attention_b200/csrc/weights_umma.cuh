@@ -29,17 +29,17 @@ using weights_tc::as_log2;
 using weights_tc::kLn2;
 using weights_tc::kLog2e;
 using weights_tc::kLowest;
-using weights_tc::RowInfo;
 
 constexpr int kThreads = 256;
 constexpr int kTile = 128;              // places, and query rows, of a tile
 constexpr int kBlockBytes = kTile * 128;  // 128 rows of 64 FP16: one swizzled block
 constexpr uint32_t kColumns = 256;      // TMEM: two accumulators of 128 columns
+constexpr int kMostSlots = 512;         // selected blocks that a CTA's run of places may touch
 
 struct Job {
   WeightsArgs a;
   int rows;            // query rows a KV head
-  int row0;            // the first of this launch, which takes up to kTile
+  int row0;            // the first of this launch's: CTAs (., ., z) take kTile from row0 + z kTile on
   int total_tiles, tiles_per_cta;
   int parts;           // parts per row in scratch (0: log-sum-exps given)
   int add;             // add to what out holds
@@ -85,7 +85,7 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
-// 32 columns of this warp's 32 lanes.
+// 32 columns of this warp's 32 lanes; the values are there after tmem_wait.
 __device__ __forceinline__ void tmem_load32(uint32_t tmem, float (&v)[32]) {
   uint32_t* r = reinterpret_cast<uint32_t*>(v);
   asm volatile(
@@ -98,7 +98,12 @@ __device__ __forceinline__ void tmem_load32(uint32_t tmem, float (&v)[32]) {
         "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
         "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(tmem));
+}
+// Waits for the loads so far. It takes their values through, so that nothing uses them before.
+__device__ __forceinline__ void tmem_wait(float (&v)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) asm volatile("" : "+f"(v[i]));
 }
 
 // Address of 16-byte chunk `chunk` (of 8) of row `row` of a swizzled block.
@@ -114,16 +119,17 @@ __global__ void __launch_bounds__(kThreads, 2) weights_umma_kernel(const Job j, 
   constexpr int kBlocks = (D + 63) / 64;        // swizzled blocks of a tile's row of FP16
   constexpr int kKeyTerms = BITS == 4 ? 2 : 1, kQueryTerms = LO ? 2 : 1;
   constexpr int kPieces = D / 32;               // 32-dim pieces of a row
-  constexpr int kOwn = (kPieces + 1) / 2;       // of them, a thread's: warp / 4, warp / 4 + 2
+  constexpr int kOwn = (kPieces + 1) / 2;       // of them, a thread's: the first ones or the rest
   constexpr int kWords = BITS;                  // 32-bit words of codes of a piece
   extern __shared__ uint8_t raw_smem[];
   __shared__ uint64_t done_bar;
   __shared__ uint32_t tmem_at;
   __shared__ int gave_up;
-  __shared__ alignas(16) RowInfo infos[kTile];
+  __shared__ alignas(16) float4 infos[kTile / 2];  // of two rows: factors, negated log-sum-exps
   __shared__ alignas(16) int seen[kTile];
   __shared__ float halves[2][kTile];
   __shared__ float2 state[kTile];
+  __shared__ int2 slots[kMostSlots];  // (pool block, valid rows) of the run's selected blocks
   __shared__ uint32_t valid_mask[4][4];  // of tile i: [i & 3] (a warp may be a tile behind another)
   const WeightsArgs& a = j.a;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quarter = warp & 3, half = warp >> 2;
@@ -134,7 +140,8 @@ __global__ void __launch_bounds__(kThreads, 2) weights_umma_kernel(const Job j, 
   const int places = a.n_sel * a.bt;
   const int first_tile = blockIdx.x * j.tiles_per_cta;
   const int tiles = min(j.total_tiles - first_tile, j.tiles_per_cta);
-  const int rows = min(kTile, j.rows - j.row0);           // query rows of this launch
+  const int row0 = j.row0 + blockIdx.z * kTile;
+  const int rows = min(kTile, j.rows - row0);               // query rows of this CTA
   const int columns = LSE ? kTile : (rows + 31) / 32 * 32;  // of the accumulator
 
   if (threadIdx.x == 0) {
@@ -148,8 +155,10 @@ __global__ void __launch_bounds__(kThreads, 2) weights_umma_kernel(const Job j, 
   pdl_launch();
 
   // ---- codes and scales of this thread's place, a tile ahead
+  const int first_slot = divide(first_tile * kTile, bt_by);
   uint32_t code[kOwn][kWords];
-  uint32_t scale[kOwn];  // of the piece's two halves of 16 dims
+  uint32_t pair_scales = 0;  // of the pieces, 16 bits each
+  const int pieces_per = a.group / 32;
   bool valid = false;
   float prev = 0.f;
   const auto load = [&](int i) {
@@ -158,35 +167,38 @@ __global__ void __launch_bounds__(kThreads, 2) weights_umma_kernel(const Job j, 
     const int place = (first_tile + i) * kTile + row;
     if (place >= places) return;
     const int slot = divide(place, bt_by), in_block = place - slot * a.bt;
-    const int blk = a.table ? a.table[slot] : slot;
-    if (blk < 0 || blk >= a.n_pool) {
-      if (a.status) atomicOr(a.status, kDevBadBlockIndex);
-    } else {
-      const int count = a.valid[blk];
-      if ((count < 0 || count > a.bt) && a.status) atomicOr(a.status, kDevBadValidCount);
-      valid = in_block < count;
-    }
+    const int2 info = slots[slot - first_slot];
+    const int blk = info.x;
+    valid = in_block < info.y;
     if (!LSE && half == 0 && (a.previous || j.add))
       prev = j.add ? a.out[h * a.out_stride + place] : a.previous[h * a.previous_stride + place];
     if (!valid) return;
     const long long r = (static_cast<long long>(blk) * a.bt + in_block) * a.kvh + h;
     const uint8_t* from = a.kp + r * (D * BITS / 8);
     const __half* s = a.ks + r * groups;
+    if constexpr (BITS == 2 && D == 128) {  // both pieces in one access
+      const uint4 v = *reinterpret_cast<const uint4*>(from + half * 16);
+      code[0][0] = v.x, code[0][1] = v.y, code[1][0] = v.z, code[1][1] = v.w;
+    } else {
 #pragma unroll
-    for (int k = 0; k < kOwn; ++k) {
-      const int piece = half + 2 * k;
-      if (piece >= kPieces) continue;
-      if constexpr (BITS == 4) {
-        const uint4 v = *reinterpret_cast<const uint4*>(from + piece * 16);
-        code[k][0] = v.x, code[k][1] = v.y, code[k][2] = v.z, code[k][3] = v.w;
-      } else {
-        const uint2 v = *reinterpret_cast<const uint2*>(from + piece * 8);
-        code[k][0] = v.x, code[k][1] = v.y;
+      for (int k = 0; k < kOwn; ++k) {
+        const int piece = half * kOwn + k;
+        if (piece >= kPieces) continue;
+        if constexpr (BITS == 4) {
+          const uint4 v = *reinterpret_cast<const uint4*>(from + piece * 16);
+          code[k][0] = v.x, code[k][1] = v.y, code[k][2] = v.z, code[k][3] = v.w;
+        } else {
+          const uint2 v = *reinterpret_cast<const uint2*>(from + piece * 8);
+          code[k][0] = v.x, code[k][1] = v.y;
+        }
       }
+    }
+    if (kOwn == 2 && D == 128 && groups == kPieces) {  // a scale a piece: two in one access
+      pair_scales = *reinterpret_cast<const uint32_t*>(s + half * 2);
+    } else {
       const unsigned short* u = reinterpret_cast<const unsigned short*>(s);
-      const int g0 = 32 * piece / a.group, g1 = (32 * piece + 16) / a.group;
-      scale[k] = u[g0];
-      scale[k] |= g1 == g0 ? scale[k] << 16 : static_cast<uint32_t>(u[g1]) << 16;
+      pair_scales = u[half * kOwn / pieces_per];
+      if (kOwn == 2) pair_scales |= static_cast<uint32_t>(u[min(half * kOwn + 1, kPieces - 1) / pieces_per]) << 16;
     }
   };
   // Dequantizes the loaded codes into the key blocks, `down` = 2^-4 where a scale is too large. Returns
@@ -196,12 +208,12 @@ __global__ void __launch_bounds__(kThreads, 2) weights_umma_kernel(const Job j, 
     if (!valid) return large;
 #pragma unroll
     for (int k = 0; k < kOwn; ++k) {
-      const int piece = half + 2 * k;
+      const int piece = half * kOwn + k;
       if (piece >= kPieces) continue;
       constexpr uint32_t kLimit = BITS == 4 ? 0x6FFFu : 0x77FFu;
-      large |= (scale[k] & 0x7FFFu) > kLimit || (scale[k] >> 16 & 0x7FFFu) > kLimit;
-      const __half2 two = __hmul2(u32_as_h2(scale[k]), down);
-      const __half2 s0 = __low2half2(two), s1 = __high2half2(two);
+      const uint32_t bits = pair_scales >> (16 * k) & 0xFFFFu;
+      large |= (bits & 0x7FFFu) > kLimit;
+      const __half2 s = __hmul2(u32_as_h2(bits * 0x10001u), down);
       const uint32_t block = keys + (piece >> 1) * kBlockBytes;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {  // 8 dims
@@ -214,7 +226,6 @@ __global__ void __launch_bounds__(kThreads, 2) weights_umma_kernel(const Job j, 
 #pragma unroll
           for (int i = 0; i < 4; ++i) o[i] = all[4 * (w & 1) + i];
         }
-        const __half2 s = w < 2 ? s0 : s1;
         uint32_t hi[4], lo[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -230,12 +241,27 @@ __global__ void __launch_bounds__(kThreads, 2) weights_umma_kernel(const Job j, 
     return large;
   };
   const __half2 kOne = __float2half2_rn(1.f), kDown = __float2half2_rn(0.0625f);
+  {
+    const int last_slot = divide(min((first_tile + tiles) * kTile, places) - 1, bt_by);
+    for (int i = threadIdx.x; i <= last_slot - first_slot; i += kThreads) {
+      const int blk = a.table ? a.table[first_slot + i] : first_slot + i;
+      int count = 0;
+      if (blk < 0 || blk >= a.n_pool) {
+        if (a.status) atomicOr(a.status, kDevBadBlockIndex);
+      } else {
+        count = a.valid[blk];
+        if ((count < 0 || count > a.bt) && a.status) atomicOr(a.status, kDevBadValidCount);
+      }
+      slots[i] = make_int2(blk, count);
+    }
+    __syncthreads();
+  }
   load(0);
 
   // ---- the query rows: two threads a row, taking turns at its units of 16 dims; their infos
   {
     constexpr int kUnits = D / 16, kMine = (kUnits + 1) / 2;
-    const int r = threadIdx.x >> 1, side = threadIdx.x & 1, at = j.row0 + r;
+    const int r = threadIdx.x >> 1, side = threadIdx.x & 1, at = row0 + r;
     const bool live = r < rows;
     const int t = live ? at / gqa : 0, head = h * gqa + (live ? at % gqa : 0);
     const long long q = (static_cast<long long>(t) * a.qh + head) * D;
@@ -308,7 +334,9 @@ __global__ void __launch_bounds__(kThreads, 2) weights_umma_kernel(const Job j, 
       if (n <= 0) l2 = INFINITY;
     }
     if (side == 0) {
-      infos[r] = {factor, l2};
+      float* pair = reinterpret_cast<float*>(infos + r / 2) + (r & 1);
+      pair[0] = factor;
+      pair[2] = -l2;
       seen[r] = n;
     }
   }
@@ -337,12 +365,14 @@ __global__ void __launch_bounds__(kThreads, 2) weights_umma_kernel(const Job j, 
   // to be multiplied by 16. `stop`: some thread's wait has run out (`timed_out`); the second barrier of
   // the rare path keeps the flag as it is until all have read it.
   bool mine_valid = false, stop = false;
+  float mine_prev = 0.f;
   const auto advance = [&](int i, bool timed_out) {
     bool large = false;
     mine_valid = valid;
     if (timed_out) gave_up = 1;
     if (i < tiles) {
       large = unpack(kOne);
+      mine_prev = prev;
       const uint32_t mask = __ballot_sync(0xffffffffu, valid);
       if (half == 0 && lane == 0) valid_mask[i & 3][quarter] = mask;
     }
@@ -361,7 +391,7 @@ __global__ void __launch_bounds__(kThreads, 2) weights_umma_kernel(const Job j, 
   };
   bool next_large = advance(0, false);
   bool next_valid = mine_valid;
-  float next_prev = prev;
+  float next_prev = mine_prev;
   load(1);
   int all_see = 0x7fffffff;  // places below are seen by every row that sees anything
   for (int i = lane; i < rows; i += 32)
@@ -369,7 +399,7 @@ __global__ void __launch_bounds__(kThreads, 2) weights_umma_kernel(const Job j, 
   all_see = __reduce_min_sync(0xffffffffu, all_see);
   if (all_see == 0x7fffffff && a.visible) all_see = 0;
 
-  const RowInfo own = infos[row];
+  const float own_factor = reinterpret_cast<const float*>(infos + row / 2)[row & 1];
   const int own_seen = seen[row];
   const uint32_t lanes_at = static_cast<uint32_t>(quarter * 32) << 16;
   float run_m = kLowest, run_l = 0.f;  // LSE: of query row `row` over this half of the columns
@@ -383,7 +413,7 @@ __global__ void __launch_bounds__(kThreads, 2) weights_umma_kernel(const Job j, 
     const float place_prev = next_prev;
     next_large = advance(i + 1, timed_out);
     next_valid = mine_valid;
-    next_prev = prev;
+    next_prev = mine_prev;
     if (stop) break;  // all threads
     if (!LSE && half == 0 && i > 0) {  // the other half of the last tile's columns has arrived
       const int place = (first_tile + i - 1) * kTile + row;
@@ -396,11 +426,14 @@ __global__ void __launch_bounds__(kThreads, 2) weights_umma_kernel(const Job j, 
     if constexpr (LSE) {
       const uint32_t* mask = valid_mask[i & 3] + 2 * half;
       const bool full = (mask[0] & mask[1]) == 0xFFFFFFFFu && place0 + kTile <= all_see;
-      const float scaled = large ? own.factor * 16.f : own.factor;
+      const float scaled = large ? own_factor * 16.f : own_factor;
+      float both[2][32];
+      tmem_load32(acc + half * 64, both[0]);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        float v[32];
-        tmem_load32(acc + half * 64 + c * 32, v);
+        float (&v)[32] = both[c];
+        tmem_wait(v);
+        if (c == 0) tmem_load32(acc + half * 64 + 32, both[1]);  // while these are worked on
         if (!full) {
           const int see = own_seen - (place0 + half * 64 + c * 32);  // columns seen
           const uint32_t live = mask[c] & (see <= 0 ? 0u : see >= 32 ? 0xFFFFFFFFu : (1u << see) - 1u);
@@ -408,47 +441,56 @@ __global__ void __launch_bounds__(kThreads, 2) weights_umma_kernel(const Job j, 
           for (int k = 0; k < 32; ++k) v[k] = live >> k & 1u ? v[k] * scaled : -INFINITY;
         }
         const float factor = full ? scaled : 1.f;
-        float top = v[0];
+        float tops[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-        for (int k = 1; k < 32; ++k) top = fmaxf(top, v[k]);
-        top *= factor;
+        for (int k = 4; k < 32; ++k) tops[k & 3] = fmaxf(tops[k & 3], v[k]);
+        const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * factor;
         if (top > run_m + 8.f) {  // the running max moves only past 2^8: terms stay finite
           run_l *= fast_exp2(run_m - top);
           run_m = top;
         }
-        float part[4] = {};
+        F2 part[2] = {f2(0.f), f2(0.f)};
+        const F2 by = f2(factor), less = f2(-run_m);
 #pragma unroll
-        for (int k = 0; k < 32; ++k) part[k & 3] += fast_exp2(fmaf(v[k], factor, -run_m));
-        run_l += (part[0] + part[1]) + (part[2] + part[3]);
+        for (int k = 0; k < 32; k += 2) {
+          const float2 x = parts(fma2(f2(v[k], v[k + 1]), by, less));
+          part[k / 2 & 1] = add2(part[k / 2 & 1], f2(fast_exp2(x.x), fast_exp2(x.y)));
+        }
+        const float2 both_sums = parts(add2(part[0], part[1]));
+        run_l += both_sums.x + both_sums.y;
       }
     } else {
       const bool full = place0 + kTile <= all_see;
-      float part[4] = {};
+      F2 part[2] = {f2(0.f), f2(0.f)};
       // the columns' chunks of 32 alternate between the halves
-      for (int c = half * 32; c < columns; c += 64) {
-        float v[32];
-        tmem_load32(acc + c, v);
+      float both[2][32];
+      if (half * 32 < columns) tmem_load32(acc + half * 32, both[0]);
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const int c = half * 32 + n * 64;
+        if (c >= columns) break;
+        float (&v)[32] = both[n];
+        tmem_wait(v);
+        if (n == 0 && c + 64 < columns) tmem_load32(acc + c + 64, both[1]);  // while these are worked on
         if (large) {
 #pragma unroll
           for (int k = 0; k < 32; ++k) v[k] *= 16.f;
         }
-        const float4* info = reinterpret_cast<const float4*>(infos + c);
-        if (full) {
+        const float4* info = infos + c / 2;
+        const int place = place0 + row;
 #pragma unroll
-          for (int k = 0; k < 32; k += 2) {
-            const float4 two = info[k / 2];
-            part[k & 3] += fast_exp2(fmaf(v[k], two.x, -two.y));
-            part[(k & 3) + 1] += fast_exp2(fmaf(v[k + 1], two.z, -two.w));
+        for (int k = 0; k < 32; k += 2) {
+          const float4 two = info[k / 2];
+          float2 x = parts(fma2(f2(v[k], v[k + 1]), f2(two.x, two.y), f2(two.z, two.w)));
+          if (!full) {
+            if (place >= seen[c + k]) x.x = -INFINITY;
+            if (place >= seen[c + k + 1]) x.y = -INFINITY;
           }
-        } else {
-#pragma unroll
-          for (int k = 0; k < 32; ++k) {
-            const RowInfo one = infos[c + k];
-            if (place0 + row < seen[c + k]) part[k & 3] += fast_exp2(fmaf(v[k], one.factor, -one.lse2));
-          }
+          part[k / 2 & 1] = add2(part[k / 2 & 1], f2(fast_exp2(x.x), fast_exp2(x.y)));
         }
       }
-      sum = place_valid ? (part[0] + part[1]) + (part[2] + part[3]) : 0.f;
+      const float2 sums = parts(add2(part[0], part[1]));
+      sum = place_valid ? sums.x + sums.y : 0.f;
       sum_prev = place_prev;
       if (half == 1) halves[i & 1][row] = sum;
     }
@@ -476,7 +518,7 @@ __global__ void __launch_bounds__(kThreads, 2) weights_umma_kernel(const Job j, 
       float2 part = make_float2(top, run_l * fast_exp2(run_m - top) + other.y * fast_exp2(other.x - top));
       if (own_seen <= 0) part = make_float2(kLowest, 0.f);
       if (stop) part = make_float2(0.f, __int_as_float(0x7fffffff));
-      reinterpret_cast<float2*>(a.scratch)[(static_cast<long long>(h) * j.rows + j.row0 + row) * j.parts +
+      reinterpret_cast<float2*>(a.scratch)[(static_cast<long long>(h) * j.rows + row0 + row) * j.parts +
                                            blockIdx.x] = part;
     }
   } else if (half == 0 && !stop) {
@@ -497,9 +539,12 @@ cudaError_t launch_pass(Job j, cudaStream_t s) {
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   const int ctas = (j.total_tiles + j.tiles_per_cta - 1) / j.tiles_per_cta;
-  for (j.row0 = 0; j.row0 < j.rows; j.row0 += kTile) {
+  const int chunks = (j.rows + kTile - 1) / kTile;
+  // log-sum-exps of different rows are independent; the weights of later rows add to those before
+  const int z = LSE && chunks <= 65535 ? chunks : 1;
+  for (j.row0 = 0; j.row0 < j.rows; j.row0 += z * kTile) {
     j.add = j.row0 > 0;
-    const cudaError_t l = launch_pdl(kernel, dim3(ctas, j.a.kvh), kThreads, smem, s, j,
+    const cudaError_t l = launch_pdl(kernel, dim3(ctas, j.a.kvh, z), kThreads, smem, s, j,
                                      divisor(static_cast<unsigned>(j.a.bt)));
     if (l != cudaSuccess) return l;
   }
@@ -514,6 +559,9 @@ cudaError_t launch(const WeightsArgs& a, cudaStream_t s) {
   j.total_tiles = static_cast<int>((static_cast<long long>(a.n_sel) * a.bt + kTile - 1) / kTile);
   const int want = 148 * 2 / a.kvh < 1 ? 1 : 148 * 2 / a.kvh;
   j.tiles_per_cta = (j.total_tiles + want - 1) / want;
+  // a run touches at most this many blocks (a partial one at either end): more CTAs otherwise
+  const long long most = static_cast<long long>(kMostSlots - 2) * a.bt / kTile;
+  if (j.tiles_per_cta > most) j.tiles_per_cta = most < 1 ? 1 : static_cast<int>(most);
   if (!a.lse_in) {
     j.parts = (j.total_tiles + j.tiles_per_cta - 1) / j.tiles_per_cta;
     const cudaError_t e = launch_pass<BITS, D, LO, true>(j, s);
