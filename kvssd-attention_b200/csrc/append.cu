@@ -234,14 +234,20 @@ struct alignas(16) Eight {
 // around through shared memory, then stay in registers over the heads; a rotation's other element comes
 // from a lane of the same row (half layout) or is the lane's own (interleaved). kGroupLanes: the lanes
 // of a scale group, 0: any number of them.
-template <typename T, int BITS, bool INTERLEAVED, int kIters, int kGroupLanes>
-__global__ void __launch_bounds__(kThreads, kIters == 4 && sizeof(T) == 2 ? 3 : 2) append_rows_kernel(const AppendArgs a, int chunks, unsigned per_lane) {
+// TURNS: whether a task's keys may be rotated; the kernel without it needs half the registers.
+constexpr int resident(int iters, int bytes, bool turns) {
+  return turns ? (iters == 4 && bytes == 2 ? 3 : 2) : (bytes == 2 ? 4 : 3);
+}
+
+template <typename T, int BITS, bool INTERLEAVED, int kIters, int kGroupLanes, bool TURNS>
+__global__ void __launch_bounds__(kThreads, resident(kIters, sizeof(T), TURNS))
+    append_rows_kernel(const AppendArgs a, int chunks, unsigned per_lane, int kv0) {
   extern __shared__ Turn turns[];  // [warps][pairs]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int lanes = a.d >> 3;                                   // of a row
   const int rows = 32u * per_lane >> 16, row = lane * per_lane >> 16;  // of a warp; this lane's
   const int l = lane - row * lanes;
-  const int kv = static_cast<int>(blockIdx.y) >= chunks, chunk = blockIdx.y - kv * chunks;
+  const int later = static_cast<int>(blockIdx.y) >= chunks, kv = kv0 + later, chunk = blockIdx.y - later * chunks;
   const int token = blockIdx.x * (kThreads / 32) + warp;
   const int pairs = a.freq ? a.pairs : 0;
   pdl_wait();
@@ -259,7 +265,7 @@ __global__ void __launch_bounds__(kThreads, kIters == 4 && sizeof(T) == 2 ? 3 : 
     else data[i] = {};
   }
   const long long slot = pool_row(a, index_at(a.slots, token));
-  if (blockIdx.y == 0 && lane == 0 && slot >= 0 && a.valid) {
+  if (kv == 0 && chunk == 0 && lane == 0 && slot >= 0 && a.valid) {
     // below 2^32 rows (nearly always) the division is the short one
     const long long block = slot >> 32 ? slot / a.bt : static_cast<unsigned>(slot) / static_cast<unsigned>(a.bt);
     atomicMax(a.valid + block, static_cast<int>(slot - block * a.bt) + 1);
@@ -269,7 +275,7 @@ __global__ void __launch_bounds__(kThreads, kIters == 4 && sizeof(T) == 2 ? 3 : 
   // behind the rotated part
   F2 ch[4], cl[4], sh[4], sl[4];
   int other = lane;  // the lane that holds the pairs' other elements: half layout
-  const bool turning = kv == 0 && pairs > 0;  // the same for the whole warp
+  const bool turning = TURNS && kv == 0 && pairs > 0;  // the same for the whole warp
   if (turning) {
     Turn* mine = turns + warp * pairs;
     const long long position = index_at(a.positions, token);
@@ -375,14 +381,23 @@ cudaError_t launch_rows(const AppendArgs& a, cudaStream_t s) {
   const int long_chunks = (a.kvh + 4 * rows - 1) / (4 * rows), short_chunks = (a.kvh + rows - 1) / rows;
   const bool few = 2ll * a.tokens * long_chunks < 148 * 16;
   const int chunks = few ? short_chunks : long_chunks;
-  const size_t smem = a.freq ? static_cast<size_t>(warps) * a.pairs * sizeof(Turn) : 0;
-  auto kernel = few ? append_rows_kernel<T, BITS, INTERLEAVED, 1, 0> : append_rows_kernel<T, BITS, INTERLEAVED, 4, 0>;
-  if (a.group == 32)
-    kernel = few ? append_rows_kernel<T, BITS, INTERLEAVED, 1, 4> : append_rows_kernel<T, BITS, INTERLEAVED, 4, 4>;
   // lane / lanes as a product: 2^16 / lanes rounded up is exact for 32 lanes
   const unsigned per_lane = (65536u + a.d / 8 - 1) / (a.d / 8);
-  return launch_pdl(kernel, dim3((a.tokens + warps - 1) / warps, 2 * chunks), kThreads, smem, s, a, chunks,
-                    per_lane);
+  const dim3 both((a.tokens + warps - 1) / warps, 2 * chunks), one(both.x, chunks);
+  const size_t smem = a.freq ? static_cast<size_t>(warps) * a.pairs * sizeof(Turn) : 0;
+  const bool g32 = a.group == 32;
+  if (few)
+    return launch_pdl(g32 ? append_rows_kernel<T, BITS, INTERLEAVED, 1, 4, true>
+                          : append_rows_kernel<T, BITS, INTERLEAVED, 1, 0, true>,
+                      both, kThreads, smem, s, a, chunks, per_lane, 0);
+  // Many tokens: values (and keys that do not turn) in a launch of their own, with more warps on an SM
+  // (8192 tokens: 22.5 us, in one launch 26.4).
+  const auto plain = g32 ? append_rows_kernel<T, BITS, false, 4, 4, false> : append_rows_kernel<T, BITS, false, 4, 0, false>;
+  const cudaError_t e = launch_pdl(plain, a.freq ? one : both, kThreads, 0, s, a, chunks, per_lane, a.freq ? 1 : 0);
+  if (e != cudaSuccess || !a.freq) return e;
+  return launch_pdl(g32 ? append_rows_kernel<T, BITS, INTERLEAVED, 4, 4, true>
+                        : append_rows_kernel<T, BITS, INTERLEAVED, 4, 0, true>,
+                    one, kThreads, smem, s, a, chunks, per_lane, 0);
 }
 
 // Whether append_rows_kernel takes this call.
@@ -393,6 +408,7 @@ bool by_rows(const AppendArgs& a) {
                        reinterpret_cast<uintptr_t>(a.packed[0]) | reinterpret_cast<uintptr_t>(a.packed[1]);
   const long long strides = a.key.token | a.key.head | a.value.token | a.value.head;
   if (at % 16 || strides * static_cast<long long>(sizeof(T)) % 16 || a.d % 8 || a.group % 8) return false;
+  if (a.kvh > 16384) return false;  // the grid's second dimension
   return !a.freq || a.pairs % (a.interleaved ? 4 : 8) == 0;
 }
 
