@@ -368,8 +368,9 @@ KVSSD_B200_API int kvssd_b200_dequantize(const uint8_t* packed, const uint16_t* 
  * weight each cached token gets, and eviction by it. Index arrays are int32, or int64 where the
  * argument beside them is nonzero; strides are in elements and the last dimension is contiguous;
  * `device_status` (NULL, or the status word of a workspace: see kvssd_b200_read_status) is OR-ed with
- * 1 for a slot or block-table entry outside the pool (skipped) and 2 for a valid count outside
- * [0, block_tokens] (clamped). Calls of one operator share no state: they may overlap on several
+ * 1 for a slot or block-table entry outside the pool (skipped), 2 for a valid count outside
+ * [0, block_tokens] (clamped) and 32 for a wait of the attention-weights kernels that gave up after
+ * about a second (their outputs are NaN then). Calls of one operator share no state: they may overlap on several
  * streams as long as their buffers differ. head_dim is at most 256. */
 
 /* Rotary positions of x [tokens, heads, head_dim] (KVSSD_B200_Q_F32 / _F16 / _BF16) into `out` of the
@@ -391,10 +392,10 @@ KVSSD_B200_API int kvssd_b200_rotary(const void* x, int dtype, long long x_token
  * equal ones the row holds a mixture). With `frequencies` (else NULL) the keys are rotated first, as
  * kvssd_b200_rotary does but rounded to FP32 once and not to their type. Codes and scales are those
  * of quantize_tensor (src/kvssd/quant.py:49-65), bit for bit, as KVCacheStore.create stores them
- * (src/kvssd/store.py:50-59); a NaN or an infinity makes
- * its group's scale NaN or infinite, and the group's codes are unspecified. Where `valid_tokens` is not NULL the
- * counts of the written blocks are raised to cover the written rows. key_values and value_values
- * (both or neither NULL) receive the FP16 values that the cache now holds for the tokens,
+ * (src/kvssd/store.py:50-59); a NaN or an infinity makes its group's scale NaN or infinite, and the
+ * group's codes are unspecified. Where `valid_tokens` is not NULL the counts of the written blocks
+ * are raised to cover the written rows. key_values and value_values (both or neither NULL) receive
+ * the FP16 values that the cache now holds for the tokens,
  * [tokens, kv_heads, head_dim] (dequantize_tensor, src/kvssd/quant.py:68-73), skipped tokens
  * included. */
 KVSSD_B200_API int kvssd_b200_append(const void* key, const void* value, int dtype,

@@ -363,6 +363,62 @@ def test_weights_windows(case, name):
     check_weights(query, kp, ks, valid, bits, group, 0.0, visible=visible, got=zero)
 
 
+SMALL_WINDOWS = [  # nb, bt, kvh, gqa, d, bits, group, queries: 9 to 32 rows, or shapes without tcgen05
+    (3, 128, 2, 4, 128, 4, 32, 7), (3, 60, 1, 3, 128, 2, 32, 10), (4, 33, 2, 5, 64, 4, 64, 2),
+    (4, 33, 3, 1, 64, 2, 32, 30), (3, 50, 2, 3, 96, 4, 96, 4), (3, 50, 2, 3, 96, 2, 48, 9),
+    (2, 128, 1, 4, 256, 4, 64, 20), (3, 40, 2, 2, 256, 2, 256, 25), (2, 128, 2, 4, 128, 4, 16, 30),
+    (2, 128, 2, 4, 64, 2, 16, 30), (2, 20, 1, 2, 256, 4, 16, 100), (3, 16, 1, 1, 128, 2, 16, 300)]
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("case", SMALL_WINDOWS)
+def test_weights_small_windows(case, name):
+    nb, bt, kvh, gqa, d, bits, group, queries = case
+    g = gen(sum(case))
+    kp, ks = key_pool(nb, bt, kvh, d, bits, group, 7, outliers=bits == 2)
+    query = (torch.randn(queries, kvh * gqa, d, generator=g) * 1.3).to(TYPES[name]).to(DEV)
+    valid = torch.full((nb,), bt, dtype=torch.int32, device=DEV)
+    valid[-1] = bt // 2
+    visible = (nb * bt - bt // 2 - queries + 1 + torch.arange(queries)).clamp_min(0).int().to(DEV)
+    previous = torch.rand(kvh, nb * bt, generator=g).to(DEV)
+    scale = 1 / math.sqrt(d)
+    got = ops.attention_weights(query, kp, ks, valid, bits, group, scale, visible=visible, previous=previous)
+    check_weights(query, kp, ks, valid, bits, group, scale, visible=visible, previous=previous, got=got)
+    lse = got[1] - 0.25
+    got = ops.attention_weights(query, kp, ks, valid, bits, group, scale, lse=lse)
+    check_weights(query, kp, ks, valid, bits, group, scale, lse=lse, got=got)
+
+
+def test_windows_in_graphs_and_on_two_streams():
+    """The tensor-memory kernel beside itself: two captured windows replayed on two streams."""
+    kp, ks = key_pool(12, 128, 4, 128, 4, 32, 2)
+    valid = torch.full((12,), 128, dtype=torch.int32, device=DEV)
+    queries = [torch.randn(40, 16, 128, generator=gen(i)).half().to(DEV) for i in range(2)]
+    call = lambda q: ops.attention_weights(q, kp, ks, valid, 4, 32, 0.09)  # noqa: E731
+    ref = [[t.clone() for t in call(q)] for q in queries]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call(queries[0])
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for q in queries:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            outs.append(call(q))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(5):
+        for s, graph in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+                graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(ref, outs):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
+    assert ops.read_device_status_all(DEV) == 0
+
+
 @pytest.mark.parametrize("bits", [2, 4])
 @pytest.mark.parametrize("queries", [1, 16])
 def test_weights_scales_at_the_end_of_fp16(bits, queries):
