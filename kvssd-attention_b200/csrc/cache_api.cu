@@ -42,7 +42,7 @@ int check_cache(int n_pool, int bt, int kvh, int d, int bits, int group) {
 
 int check_places(int n_sel, int bt) {
   if (n_sel < 1) return bad("at least one block is required");
-  if (static_cast<long long>(n_sel) * bt > 0x7fffff00ll)
+  if (static_cast<long long>(n_sel) * bt > 0x7ff00000ll)  // room for a tile or batch behind the last
     return report(KVSSD_B200_ERR_UNSUPPORTED, "more than 2^31 places are not supported");
   return KVSSD_B200_OK;
 }
@@ -150,7 +150,7 @@ int kvssd_b200_attention_weights(const void* query, int query_dtype, int queries
 int kvssd_b200_evict_scratch_size(int n_tokens, int keep, int kv_heads, int shared, size_t* bytes) {
   if (!bytes) return bad("bytes must not be NULL");
   if (n_tokens < 1 || keep < 0 || keep > n_tokens || kv_heads < 1) return bad("bad eviction sizes");
-  *bytes = sizeof(int32_t) * (static_cast<size_t>(n_tokens) + 1) * (shared ? 1 : kv_heads);
+  *bytes = sizeof(int32_t) * evict_scratch_ints(n_tokens, shared ? 1 : kv_heads);
   return KVSSD_B200_OK;
 }
 
@@ -187,6 +187,7 @@ int kvssd_b200_evict(const float* weights, long long weights_stride, const int32
   EvictArgs a{weights, weights_stride, positions, positions_stride, n_tokens, keep, columns, sink,
               recent_from, shared ? 1 : 0, new_weights, new_positions, lists_at + lists,
               lists_at + lists + static_cast<size_t>(lists) * keep, lists_at,
+              reinterpret_cast<unsigned*>(lists_at + lists + static_cast<size_t>(lists) * n_tokens),
               {packed_k, packed_v},
               {reinterpret_cast<__half*>(scales_k), reinterpret_cast<__half*>(scales_v)},
               valid_tokens, block_table, n_pool_blocks, n_sel_blocks, block_tokens, kv_heads,

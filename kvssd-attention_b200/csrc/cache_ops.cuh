@@ -91,6 +91,7 @@ struct EvictArgs {
   int32_t* holes;          // scratch [lists, keep]
   int32_t* movers;         // scratch [lists, n - keep]
   int32_t* counts;         // scratch [lists]
+  unsigned* keys;          // scratch [lists, n] of the longest caches
   uint8_t* packed[2];
   __half* scales[2];
   int32_t* valid;
@@ -107,6 +108,7 @@ cudaError_t launch_rotary(const RotaryArgs& a, cudaStream_t s);
 cudaError_t launch_append(const AppendArgs& a, cudaStream_t s);
 size_t weights_scratch_bytes(int queries, int qh, int n_sel, int bt);
 cudaError_t launch_weights(const WeightsArgs& a, cudaStream_t s);
+size_t evict_scratch_ints(int n, int lists);
 cudaError_t launch_evict(const EvictArgs& a, cudaStream_t s);
 
 // Launch with programmatic stream serialization (see above).

@@ -6,12 +6,12 @@
 // rotary position stay as they are (attention does not mind the order).
 //
 // Selection: one cluster of CTAs per choice (a KV head, or all of them). A radix select over
-// order-preserving 32-bit keys finds the smallest kept key, 8 bits a pass: each CTA counts its own run
+// order-preserving 32-bit keys finds the smallest kept key, a digit a pass: each CTA counts its own run
 // of places in shared memory, and after a cluster barrier every CTA adds up the cluster's counts
 // through distributed shared memory. A last scan in the order of the places copies the weights and
 // positions that stay and lists the places to fill and the places to move (their numbers are equal).
 // evict_select_kernel keeps each thread's run of consecutive keys in registers;
-// evict_select_long_kernel is the form for caches that do not fit. evict_move_kernel then moves the
+// evict_select_long_kernel is the form for caches that do not fit (keys in shared memory, or in scratch). evict_move_kernel then moves the
 // pool rows with their weights and positions, on all SMs.
 //
 // Bound by HBM: the weights are read once; per moved token and head two packed rows and their scales
@@ -37,20 +37,6 @@ __device__ __forceinline__ unsigned weight_key(float w) {
   if (w != w) return 0u;
   const unsigned b = __float_as_uint(w + 0.f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
-}
-
-__device__ __forceinline__ unsigned place_key(const EvictArgs& a, int list, int place) {
-  const int pos = a.positions[list * a.positions_stride + place];
-  if (pos < a.sink || pos >= a.recent_from) return 0xFFFFFFFFu;
-  float w;
-  if (a.shared) {
-    double sum = 0.0;
-    for (int h = 0; h < a.kvh; ++h) sum += static_cast<double>(a.weights[h * a.weights_stride + place]);
-    w = static_cast<float>(sum);
-  } else {
-    w = a.weights[list * a.weights_stride + place];
-  }
-  return weight_key(w);
 }
 
 // Which digit of the keys holds the `need`-th largest, and how many keys lie above it: from the
@@ -104,128 +90,6 @@ __device__ __forceinline__ Counts operator+(const Counts& x, const Counts& y) {
   return {x.above_early + y.above_early, x.equal_early + y.equal_early, x.above_late + y.above_late,
           x.equal_late + y.equal_late};
 }
-
-__global__ void __launch_bounds__(kThreads) evict_select_long_kernel(const EvictArgs a, int run, int cached) {
-  extern __shared__ unsigned keys[];  // [run] when cached
-  __shared__ unsigned hist[2][kBins];
-  __shared__ unsigned total[kBins];
-  __shared__ Counts warp_counts[kWarps];
-  __shared__ Counts cta_counts;
-  __shared__ unsigned found[2];  // digit, keys above it
-  cg::cluster_group cluster = cg::this_cluster();
-  const int rank = static_cast<int>(cluster.block_rank());
-  const int list = blockIdx.y;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int first = min(a.n, rank * run), last = min(a.n, first + run);
-
-  pdl_wait();
-  pdl_launch();
-  const auto key_at = [&](int i) { return cached ? keys[i - first] : place_key(a, list, i); };
-  if (cached)
-    for (int i = first + static_cast<int>(threadIdx.x); i < last; i += kThreads)
-      keys[i - first] = place_key(a, list, i);
-
-  // The keep-th largest key, digit by digit; `need` = how many of the keys with this prefix to keep.
-  unsigned prefix = 0, need = static_cast<unsigned>(a.keep);
-  for (int pass = 0; pass < 4; ++pass) {
-    const int shift = 24 - 8 * pass;
-    unsigned* mine = hist[pass & 1];
-    for (int b = threadIdx.x; b < kBins; b += kThreads) mine[b] = 0;
-    __syncthreads();
-    for (int i = first + static_cast<int>(threadIdx.x); i < last; i += kThreads) {
-      const unsigned k = key_at(i);
-      if (pass == 0 || (k >> (shift + 8)) == prefix) atomicAdd(&mine[k >> shift & 255u], 1u);
-    }
-    cluster.sync();
-    for (int b = threadIdx.x; b < kBins; b += kThreads) {
-      unsigned sum = 0;
-      for (int r = 0; r < kLongCluster; ++r) sum += *cluster.map_shared_rank(&mine[b], r);
-      total[b] = sum;
-    }
-    __syncthreads();
-    find_digit(total, need, found);
-    prefix = prefix << 8 | found[0];
-    need -= found[1];
-    // hist[pass & 1] is written again two passes on, behind the next pass's cluster barrier
-  }
-  const unsigned border = prefix;  // kept: keys above it, and the first `need` equal to it
-
-  // Warp w counts its own run of places, 32 at a time in their order.
-  const int per_warp = (run + kWarps * 32 - 1) / (kWarps * 32) * 32;
-  const int wfirst = min(last, first + warp * per_warp), wlast = min(last, wfirst + per_warp);
-  Counts c{0, 0, 0, 0};
-  for (int i = wfirst + lane; i - lane < wlast; i += 32) {
-    const unsigned k = i < wlast ? key_at(i) : 0u;
-    const bool in = i < wlast, early = i < a.keep;
-    c.above_early += __popc(__ballot_sync(0xffffffffu, in && early && k > border));
-    c.equal_early += __popc(__ballot_sync(0xffffffffu, in && early && k == border));
-    c.above_late += __popc(__ballot_sync(0xffffffffu, in && !early && k > border));
-    c.equal_late += __popc(__ballot_sync(0xffffffffu, in && !early && k == border));
-  }
-  if (lane == 0) warp_counts[warp] = c;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    Counts sum{0, 0, 0, 0};
-    for (int w = 0; w < kWarps; ++w) {
-      const Counts own = warp_counts[w];
-      warp_counts[w] = sum;
-      sum = sum + own;
-    }
-    cta_counts = sum;
-  }
-  cluster.sync();
-  Counts before = warp_counts[warp];
-  for (int r = 0; r < rank; ++r) before = before + *cluster.map_shared_rank(&cta_counts, r);
-
-  // Ranks in the order of the places: equal keys, places to fill, places to move.
-  int equals = before.equal_early + before.equal_late;
-  const int want = static_cast<int>(need);
-  // of the equal keys before this run the first `want` are kept; the early ones come first
-  const int kept_early = before.above_early + min(before.equal_early, want);
-  int late = before.above_late + min(equals, want) - min(before.equal_early, want);
-  int hole = min(wfirst, a.keep) - kept_early;
-  const int lists = a.shared ? a.kvh : 1;  // heads this choice is for
-  int32_t* holes = a.holes + static_cast<long long>(list) * a.keep;
-  int32_t* movers = a.movers + static_cast<long long>(list) * (a.n - a.keep);
-  for (int i = wfirst + lane; i - lane < wlast; i += 32) {
-    const bool in = i < wlast, early = i < a.keep;
-    const unsigned k = in ? key_at(i) : 0u;
-    const unsigned below = (1u << lane) - 1u;
-    const unsigned eq = __ballot_sync(0xffffffffu, in && k == border);
-    const bool kept = in && (k > border || (k == border && equals + __popc(eq & below) < want));
-    equals += __popc(eq);
-    const unsigned fill = __ballot_sync(0xffffffffu, in && early && !kept);
-    const unsigned move = __ballot_sync(0xffffffffu, kept && !early);
-    if (in && early && !kept) holes[hole + __popc(fill & below)] = i;
-    if (kept && !early) movers[late + __popc(move & below)] = i;
-    hole += __popc(fill);
-    late += __popc(move);
-    if (in)
-      for (int j = 0; j < lists; ++j) {
-        const int h = list + j;
-        const long long to = static_cast<long long>(h) * a.columns + i;
-        a.new_weights[to] = early ? a.weights[h * a.weights_stride + i] : 0.f;
-        a.new_positions[to] = early ? a.positions[h * a.positions_stride + i] : -1;
-      }
-  }
-  if (rank == kLongCluster - 1) {  // the columns behind the cache's length
-    for (int i = a.n + static_cast<int>(threadIdx.x); i < a.columns; i += kThreads)
-      for (int j = 0; j < lists; ++j) {
-        a.new_weights[static_cast<long long>(list + j) * a.columns + i] = 0.f;
-        a.new_positions[static_cast<long long>(list + j) * a.columns + i] = -1;
-      }
-    if (warp == kWarps - 1 && lane == 0) a.counts[list] = late;  // the last run's end: all movers
-    if (list == 0) write_valid_counts(a);
-  }
-  cluster.sync();  // no CTA leaves while its counts are read
-}
-
-// The same for up to cluster * kThreads * E places: each CTA has a run of up to kThreads * E of them, and
-// thread t of it holds the keys of the E places from t * E on in that run. Digits of 11, 11 and 10 bits: three rounds of counting, barrier, adding up
-// and searching at about 3 us each, of which the counting is the smallest part. The weights and
-// positions are written to their new places as soon as they are read (evict_move_kernel overwrites the
-// places to fill), and the lists go through shared memory, so that their stores are whole lines.
-constexpr int kDigits = 2048;
 
 // x in FP64, by its bits: the conversion instruction is an eighth as fast as the addition.
 __device__ __forceinline__ double widen(float x) {
@@ -310,6 +174,126 @@ __device__ __forceinline__ void load_places(const EvictArgs& a, int list, int fi
     }
   }
 }
+
+__global__ void __launch_bounds__(kThreads) evict_select_long_kernel(const EvictArgs a, int run, int cached, int vectors) {
+  extern __shared__ __align__(16) unsigned in_shared[];  // the run's keys when cached; else in scratch
+  __shared__ unsigned hist[2][kBins];
+  __shared__ unsigned total[kBins];
+  __shared__ Counts warp_counts[kWarps];
+  __shared__ Counts cta_counts;
+  __shared__ unsigned found[2];  // digit, keys above it
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = static_cast<int>(cluster.block_rank());
+  const int list = blockIdx.y;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int first = min(a.n, rank * run), last = min(a.n, first + run);
+
+  pdl_wait();
+  pdl_launch();
+  unsigned* keys = cached ? in_shared : a.keys + static_cast<long long>(list) * a.n + first;
+  if (a.shared) {
+    if (vectors) load_places<16, 4, true>(a, list, first, last, keys);
+    else load_places<16, 1, true>(a, list, first, last, keys);
+  } else {
+    if (vectors) load_places<16, 4, false>(a, list, first, last, keys);
+    else load_places<16, 1, false>(a, list, first, last, keys);
+  }
+  const auto key_at = [&](int i) { return keys[i - first]; };
+
+  // The keep-th largest key, digit by digit; `need` = how many of the keys with this prefix to keep.
+  unsigned prefix = 0, need = static_cast<unsigned>(a.keep);
+  for (int pass = 0; pass < 4; ++pass) {
+    const int shift = 24 - 8 * pass;
+    unsigned* mine = hist[pass & 1];
+    for (int b = threadIdx.x; b < kBins; b += kThreads) mine[b] = 0;
+    __syncthreads();
+    for (int i = first + static_cast<int>(threadIdx.x); i < last; i += kThreads) {
+      const unsigned k = key_at(i);
+      if (pass == 0 || (k >> (shift + 8)) == prefix) atomicAdd(&mine[k >> shift & 255u], 1u);
+    }
+    cluster.sync();
+    for (int b = threadIdx.x; b < kBins; b += kThreads) {
+      unsigned sum = 0;
+      for (int r = 0; r < kLongCluster; ++r) sum += *cluster.map_shared_rank(&mine[b], r);
+      total[b] = sum;
+    }
+    __syncthreads();
+    find_digit(total, need, found);
+    prefix = prefix << 8 | found[0];
+    need -= found[1];
+    // hist[pass & 1] is written again two passes on, behind the next pass's cluster barrier
+  }
+  const unsigned border = prefix;  // kept: keys above it, and the first `need` equal to it
+
+  // Warp w counts its own run of places, 32 at a time in their order.
+  const int per_warp = (run + kWarps * 32 - 1) / (kWarps * 32) * 32;
+  const int wfirst = min(last, first + warp * per_warp), wlast = min(last, wfirst + per_warp);
+  Counts c{0, 0, 0, 0};
+  for (int i = wfirst + lane; i - lane < wlast; i += 32) {
+    const unsigned k = i < wlast ? key_at(i) : 0u;
+    const bool in = i < wlast, early = i < a.keep;
+    c.above_early += __popc(__ballot_sync(0xffffffffu, in && early && k > border));
+    c.equal_early += __popc(__ballot_sync(0xffffffffu, in && early && k == border));
+    c.above_late += __popc(__ballot_sync(0xffffffffu, in && !early && k > border));
+    c.equal_late += __popc(__ballot_sync(0xffffffffu, in && !early && k == border));
+  }
+  if (lane == 0) warp_counts[warp] = c;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    Counts sum{0, 0, 0, 0};
+    for (int w = 0; w < kWarps; ++w) {
+      const Counts own = warp_counts[w];
+      warp_counts[w] = sum;
+      sum = sum + own;
+    }
+    cta_counts = sum;
+  }
+  cluster.sync();
+  Counts before = warp_counts[warp];
+  for (int r = 0; r < rank; ++r) before = before + *cluster.map_shared_rank(&cta_counts, r);
+
+  // Ranks in the order of the places: equal keys, places to fill, places to move.
+  int equals = before.equal_early + before.equal_late;
+  const int want = static_cast<int>(need);
+  // of the equal keys before this run the first `want` are kept; the early ones come first
+  const int kept_early = before.above_early + min(before.equal_early, want);
+  int late = before.above_late + min(equals, want) - min(before.equal_early, want);
+  int hole = min(wfirst, a.keep) - kept_early;
+  const int lists = a.shared ? a.kvh : 1;  // heads this choice is for
+  int32_t* holes = a.holes + static_cast<long long>(list) * a.keep;
+  int32_t* movers = a.movers + static_cast<long long>(list) * (a.n - a.keep);
+  for (int i = wfirst + lane; i - lane < wlast; i += 32) {
+    const bool in = i < wlast, early = i < a.keep;
+    const unsigned k = in ? key_at(i) : 0u;
+    const unsigned below = (1u << lane) - 1u;
+    const unsigned eq = __ballot_sync(0xffffffffu, in && k == border);
+    const bool kept = in && (k > border || (k == border && equals + __popc(eq & below) < want));
+    equals += __popc(eq);
+    const unsigned fill = __ballot_sync(0xffffffffu, in && early && !kept);
+    const unsigned move = __ballot_sync(0xffffffffu, kept && !early);
+    if (in && early && !kept) holes[hole + __popc(fill & below)] = i;
+    if (kept && !early) movers[late + __popc(move & below)] = i;
+    hole += __popc(fill);
+    late += __popc(move);
+  }
+  if (rank == kLongCluster - 1) {  // the columns behind the cache's length
+    for (int i = a.n + static_cast<int>(threadIdx.x); i < a.columns; i += kThreads)
+      for (int j = 0; j < lists; ++j) {
+        a.new_weights[static_cast<long long>(list + j) * a.columns + i] = 0.f;
+        a.new_positions[static_cast<long long>(list + j) * a.columns + i] = -1;
+      }
+    if (warp == kWarps - 1 && lane == 0) a.counts[list] = late;  // the last run's end: all movers
+    if (list == 0) write_valid_counts(a);
+  }
+  cluster.sync();  // no CTA leaves while its counts are read
+}
+
+// The same for up to cluster * kThreads * E places: each CTA has a run of up to kThreads * E of them, and
+// thread t of it holds the keys of the E places from t * E on in that run. Digits of 11, 11 and 10 bits: three rounds of counting, barrier, adding up
+// and searching at about 3 us each, of which the counting is the smallest part. The weights and
+// positions are written to their new places as soon as they are read (evict_move_kernel overwrites the
+// places to fill), and the lists go through shared memory, so that their stores are whole lines.
+constexpr int kDigits = 2048;
 
 template <int E>
 __global__ void __launch_bounds__(kThreads) evict_select_kernel(const EvictArgs a, int run, int vectors) {
@@ -656,15 +640,20 @@ cudaError_t select(const EvictArgs& a, int lists, cudaStream_t s) {
   if (a.n <= ranks * kThreads * 8) return select_in_registers<8>(a, ranks, lists, vectors, s);
   if (a.n <= ranks * kThreads * 16) return select_in_registers<16>(a, ranks, lists, vectors, s);
   const int run = static_cast<int>((static_cast<long long>(a.n) + kLongCluster * 32 - 1) / (kLongCluster * 32) * 32);
-  const int cached = run <= kMaxCached;
+  const int cached = run <= kMaxCached;  // evict_scratch_ints has room for the keys otherwise
   const cudaError_t e = cudaFuncSetAttribute(evict_select_long_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                              kMaxCached * sizeof(unsigned));
   if (e != cudaSuccess) return e;
   return launch_select(evict_select_long_kernel, kLongCluster, lists, cached ? run * sizeof(unsigned) : 0, s, a,
-                       run, cached);
+                       run, cached, vectors);
 }
 
 }  // namespace
+
+size_t evict_scratch_ints(int n, int lists) {
+  const size_t listed = static_cast<size_t>(lists) * (static_cast<size_t>(n) + 1);
+  return n > kLongCluster * (kMaxCached - 32) ? listed + static_cast<size_t>(lists) * n : listed;
+}
 
 cudaError_t launch_evict(const EvictArgs& a, cudaStream_t s) {
   const int lists = a.shared ? 1 : a.kvh;

@@ -1038,13 +1038,18 @@ def evict(weights: torch.Tensor, positions: torch.Tensor, n_tokens: int, keep: i
     lists = 1 if shared else kvh
     new_weights = torch.empty((kvh, columns), dtype=torch.float32, device=weights.device)
     new_positions = torch.empty((kvh, columns), dtype=torch.int32, device=weights.device)
-    scratch = torch.empty(lists * (n_tokens + 1), dtype=torch.int32, device=weights.device)
+    ints = lists * (n_tokens + 1)
+    if n_tokens > 1 << 17:  # the longest caches need more
+        need = ctypes.c_size_t()
+        _call(index, "kvssd_b200_evict_scratch_size", n_tokens, keep, kvh, shared, ctypes.byref(need))
+        ints = need.value // 4
+    scratch = torch.empty(ints, dtype=torch.int32, device=weights.device)
     stream = _raw_stream(index)
     _call(index, "kvssd_b200_evict", weights.data_ptr(), weights.stride(0), positions.data_ptr(),
           positions.stride(0), n_tokens, keep, sink, recent_from, shared, new_weights.data_ptr(),
           new_positions.data_ptr(), columns, packed_k.data_ptr(), packed_v.data_ptr(),
           scales_k.data_ptr(), scales_v.data_ptr(), valid_tokens.data_ptr(), _ptr(block_table),
-          n_pool, n_sel, bt, kvh, pd, scales[3], scratch.data_ptr(), 4 * lists * (n_tokens + 1),
+          n_pool, n_sel, bt, kvh, pd, scales[3], scratch.data_ptr(), 4 * ints,
           _status_word(index, stream), stream)
     return new_weights, new_positions
 

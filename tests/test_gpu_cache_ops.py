@@ -667,6 +667,36 @@ def test_evict_long_cache():
     np.testing.assert_array_equal(pool[0].flatten()[keep:].cpu().numpy(), np.arange(keep, nb * 128) % 251)
 
 
+@pytest.mark.parametrize("n, shared", [(150_000, True), (400_003, False), (400_000, True)])
+def test_evict_long_caches_by_head(n, shared):
+    """Long caches of two heads, with and without vector accesses, against a sort."""
+    nb = -(-n // 64)
+    w, pos = stats(2, nb * 64, n, n, mixed=True, shared=shared)
+    pool = [torch.randint(0, 256, (nb, 64, 2, 4), generator=gen(1), dtype=torch.uint8) for _ in "kv"] + [
+        torch.rand(nb, 64, 2, 1, generator=gen(2)).half() for _ in "kv"]
+    dev = [t.to(DEV) for t in pool]
+    valid = torch.zeros(nb, dtype=torch.int32, device=DEV)
+    keep = n // 3
+    new_w, new_p = ops.evict(w.to(DEV), pos.to(DEV), n, keep, *dev, valid, sink=3, recent=77, shared=shared)
+    total = w[:, :n].numpy().astype(np.float64).sum(0).astype(np.float32)
+    for h in range(2):
+        rank = total if shared else w[h, :n].numpy()
+        p = pos[h, :n].numpy()
+        order = np.lexsort((np.arange(n), -rank.astype(np.float64), ~((p < 3) | (p >= n - 77))))
+        kept = np.zeros(n, bool)
+        kept[order[:keep]] = True
+        source = np.arange(keep)
+        source[~kept[:keep]] = keep + np.nonzero(kept[keep:])[0]
+        np.testing.assert_array_equal(new_p[h, :keep].cpu().numpy(), p[source])
+        np.testing.assert_array_equal(new_w[h, :keep].cpu().numpy(), w[h].numpy()[source])
+        assert (new_p[h, keep:] == -1).all() and (new_w[h, keep:] == 0).all()
+        for got, t in zip(dev, pool):
+            flat = t.flatten(0, 1)[:, h].numpy()
+            now = got.flatten(0, 1)[:, h].cpu().numpy()
+            np.testing.assert_array_equal(now[:keep], flat[source])
+            np.testing.assert_array_equal(now[keep:], flat[keep:])
+
+
 def test_evict_refuses_blocks_outside_the_pool():
     ops.read_device_status(DEV)
     w, pos = stats(1, 32, 32, 3)
