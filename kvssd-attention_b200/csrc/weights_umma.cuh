@@ -65,6 +65,14 @@ __device__ __forceinline__ void fence_async_proxy() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
+// Waits for a phase of the MMAs' barrier, a second at most. The clock is read only when the phase is not
+// near: a read takes about as long as a tile's MMAs.
+__device__ __forceinline__ bool wait_done(uint32_t bar, uint32_t parity) {
+  for (int i = 0; i < 64; ++i)
+    if (mbar_try(bar, parity)) return true;
+  return mbar_wait_until(bar, parity, global_ns() + 1000000000ull, 1u << 26);
+}
+
 // Shared-memory matrix descriptor: K-major rows of 128 bytes with the 128-byte swizzle, groups of 8 rows
 // 1024 bytes apart.
 __device__ __forceinline__ uint64_t matrix(uint32_t addr) {
@@ -407,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, 2) weights_umma_kernel(const Job j, 
 
   int i = 0;
   for (; i < tiles; ++i) {
-    const bool timed_out = !mbar_wait_until(bar, i & 1, global_ns() + 1000000000ull, 1u << 26);
+    const bool timed_out = !wait_done(bar, i & 1);
     fence_after_sync();
     const bool large = next_large, place_valid = next_valid;
     const float place_prev = next_prev;
@@ -498,7 +506,7 @@ __global__ void __launch_bounds__(kThreads, 2) weights_umma_kernel(const Job j, 
 
   if (stop) {  // the MMAs' barrier did not complete in a second: nothing plausible is left behind
     if (threadIdx.x == 0 && a.status) atomicOr(a.status, kDevStreamTimeout);
-    mbar_wait_until(bar, i & 1, global_ns() + 1000000000ull, 1u << 26);
+    wait_done(bar, i & 1);
     const float nan = __int_as_float(0x7fffffff);
     run_l = run_m = nan;
     if (!LSE && half == 0)
