@@ -10,8 +10,8 @@ namespace weights_tc {
 
 template <int BITS, int D, int UNIT, bool LO>
 cudaError_t launch_shape(const WeightsArgs& a, cudaStream_t s) {
-  if constexpr (D <= 128 && UNIT == 32)
-    if (weights_umma::takes(a)) return weights_umma::launch<BITS, D, LO>(a, s);
+  if constexpr (D <= 128 || BITS == 2 || !LO)
+    if (weights_umma::takes<BITS, D, LO>(a)) return weights_umma::launch<BITS, D, LO>(a, s);
   Job j{};
   j.a = a;
   j.rows = a.queries * (a.qh / a.kvh);

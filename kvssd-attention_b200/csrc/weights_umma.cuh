@@ -1,5 +1,5 @@
 // Attention weights of many query rows a KV head (a prompt's window) on the 5th-generation tensor cores:
-// head_dim 64, 96 and 128.
+// head_dim 64, 96, 128 and 256, scale groups of whole 16 dims.
 //
 // Math. A tile is 128 places by up to 128 query rows. The places' keys are dequantized into shared memory
 // as FP16: a centred INT2 code times its FP16 scale is exact in FP16; an INT4 one has up to 14 bits and
@@ -16,7 +16,7 @@
 //
 // A CTA walks a run of tiles: it waits for the MMAs of tile i, unpacks tile i + 1 into the one key buffer,
 // issues its MMAs into the other half of the accumulator, and works on tile i's scores while they run. Two
-// CTAs share an SM. Codes are loaded a tile ahead into registers.
+// CTAs share an SM (one at head_dim 256). Codes are loaded a tile ahead into registers.
 #pragma once
 
 #include "tma.cuh"
@@ -122,13 +122,17 @@ __device__ __forceinline__ void store_chunk(uint32_t at, uint32_t a, uint32_t b,
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
+constexpr int resident(int d) { return d <= 128 ? 2 : 1; }  // CTAs on an SM
+
 template <int BITS, int D, bool LO, bool LSE>
-__global__ void __launch_bounds__(kThreads, 2) weights_umma_kernel(const Job j, Divisor bt_by) {
+__global__ void __launch_bounds__(kThreads, resident(D)) weights_umma_kernel(const Job j, Divisor bt_by) {
   constexpr int kBlocks = (D + 63) / 64;        // swizzled blocks of a tile's row of FP16
   constexpr int kKeyTerms = BITS == 4 ? 2 : 1, kQueryTerms = LO ? 2 : 1;
   constexpr int kPieces = D / 32;               // 32-dim pieces of a row
   constexpr int kOwn = (kPieces + 1) / 2;       // of them, a thread's: the first ones or the rest
   constexpr int kWords = BITS;                  // 32-bit words of codes of a piece
+  // both halves have whole pairs of pieces: their rows start on 16 bytes of INT2 codes, 4 of scales
+  constexpr bool kEven = kPieces % 4 == 0;
   extern __shared__ uint8_t raw_smem[];
   __shared__ uint64_t done_bar;
   __shared__ uint32_t tmem_at;
@@ -165,8 +169,10 @@ __global__ void __launch_bounds__(kThreads, 2) weights_umma_kernel(const Job j, 
   // ---- codes and scales of this thread's place, a tile ahead
   const int first_slot = divide(first_tile * kTile, bt_by);
   uint32_t code[kOwn][kWords];
-  uint32_t pair_scales = 0;  // of the pieces, 16 bits each
-  const int pieces_per = a.group / 32;
+  // Scales: in pairs, of two pieces each (groups of 32, kEven); of a piece's
+  // two halves of 16 dims (groups of 16 or 48); or one a piece.
+  uint32_t scale[kOwn];
+  const bool in_pairs = a.group == 32 && kEven, in_halves = a.group % 32 != 0;
   bool valid = false;
   float prev = 0.f;
   const auto load = [&](int i) {
@@ -184,9 +190,12 @@ __global__ void __launch_bounds__(kThreads, 2) weights_umma_kernel(const Job j, 
     const long long r = (static_cast<long long>(blk) * a.bt + in_block) * a.kvh + h;
     const uint8_t* from = a.kp + r * (D * BITS / 8);
     const __half* s = a.ks + r * groups;
-    if constexpr (BITS == 2 && D == 128) {  // both pieces in one access
-      const uint4 v = *reinterpret_cast<const uint4*>(from + half * 16);
-      code[0][0] = v.x, code[0][1] = v.y, code[1][0] = v.z, code[1][1] = v.w;
+    if constexpr (BITS == 2 && kEven) {  // two pieces in one access
+#pragma unroll
+      for (int k = 0; k < kOwn; k += 2) {
+        const uint4 v = *reinterpret_cast<const uint4*>(from + (half * kOwn + k) * 8);
+        code[k][0] = v.x, code[k][1] = v.y, code[k + 1][0] = v.z, code[k + 1][1] = v.w;
+      }
     } else {
 #pragma unroll
       for (int k = 0; k < kOwn; ++k) {
@@ -201,12 +210,18 @@ __global__ void __launch_bounds__(kThreads, 2) weights_umma_kernel(const Job j, 
         }
       }
     }
-    if (kOwn == 2 && D == 128 && groups == kPieces) {  // a scale a piece: two in one access
-      pair_scales = *reinterpret_cast<const uint32_t*>(s + half * 2);
+    const unsigned short* u = reinterpret_cast<const unsigned short*>(s);
+    if (in_pairs) {
+#pragma unroll
+      for (int k = 0; k < kOwn; k += 2) scale[k] = *reinterpret_cast<const uint32_t*>(u + half * kOwn + k);
     } else {
-      const unsigned short* u = reinterpret_cast<const unsigned short*>(s);
-      pair_scales = u[half * kOwn / pieces_per];
-      if (kOwn == 2) pair_scales |= static_cast<uint32_t>(u[min(half * kOwn + 1, kPieces - 1) / pieces_per]) << 16;
+#pragma unroll
+      for (int k = 0; k < kOwn; ++k) {
+        const int piece = min(half * kOwn + k, kPieces - 1);
+        if (a.group == 16) scale[k] = reinterpret_cast<const uint32_t*>(u)[piece];
+        else if (in_halves) scale[k] = u[32 * piece / a.group] | static_cast<uint32_t>(u[(32 * piece + 16) / a.group]) << 16;
+        else scale[k] = u[32 * piece / a.group];
+      }
     }
   };
   // Dequantizes the loaded codes into the key blocks, `down` = 2^-4 where a scale is too large. Returns
@@ -219,9 +234,11 @@ __global__ void __launch_bounds__(kThreads, 2) weights_umma_kernel(const Job j, 
       const int piece = half * kOwn + k;
       if (piece >= kPieces) continue;
       constexpr uint32_t kLimit = BITS == 4 ? 0x6FFFu : 0x77FFu;
-      const uint32_t bits = pair_scales >> (16 * k) & 0xFFFFu;
-      large |= (bits & 0x7FFFu) > kLimit;
-      const __half2 s = __hmul2(u32_as_h2(bits * 0x10001u), down);
+      const uint32_t one = in_pairs ? scale[k & ~1] >> (16 * (k & 1)) & 0xFFFFu : scale[k];
+      const uint32_t bits = in_halves ? one : one * 0x10001u;
+      large |= (bits & 0x7FFFu) > kLimit || (bits >> 16 & 0x7FFFu) > kLimit;
+      const __half2 two = __hmul2(u32_as_h2(bits), down);
+      const __half2 s0 = __low2half2(two), s1 = __high2half2(two);
       const uint32_t block = keys + (piece >> 1) * kBlockBytes;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {  // 8 dims
@@ -234,6 +251,7 @@ __global__ void __launch_bounds__(kThreads, 2) weights_umma_kernel(const Job j, 
 #pragma unroll
           for (int i = 0; i < 4; ++i) o[i] = all[4 * (w & 1) + i];
         }
+        const __half2 s = w < 2 ? s0 : s1;
         uint32_t hi[4], lo[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -536,8 +554,12 @@ __global__ void __launch_bounds__(kThreads, 2) weights_umma_kernel(const Job j, 
   if (warp == 0) tmem_free(tmem_at);
 }
 
-// Query rows from which the 128-row tiles pay.
-inline bool takes(const WeightsArgs& a) { return a.queries * (a.qh / a.kvh) > 32; }
+// Query rows from which the 128-row tiles pay; keys and queries in two terms each are too large for the
+// shared memory at head_dim 256.
+template <int BITS, int D, bool LO>
+bool takes(const WeightsArgs& a) {
+  return a.queries * (a.qh / a.kvh) > 32 && !(D == 256 && BITS == 4 && LO);
+}
 
 template <int BITS, int D, bool LO, bool LSE>
 cudaError_t launch_pass(Job j, cudaStream_t s) {
@@ -565,7 +587,7 @@ cudaError_t launch(const WeightsArgs& a, cudaStream_t s) {
   j.a = a;
   j.rows = a.queries * (a.qh / a.kvh);
   j.total_tiles = static_cast<int>((static_cast<long long>(a.n_sel) * a.bt + kTile - 1) / kTile);
-  const int want = 148 * 2 / a.kvh < 1 ? 1 : 148 * 2 / a.kvh;
+  const int want = 148 * resident(D) / a.kvh < 1 ? 1 : 148 * resident(D) / a.kvh;
   j.tiles_per_cta = (j.total_tiles + want - 1) / want;
   // a run touches at most this many blocks (a partial one at either end): more CTAs otherwise
   const long long most = static_cast<long long>(kMostSlots - 2) * a.bt / kTile;

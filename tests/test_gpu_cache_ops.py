@@ -330,7 +330,10 @@ def test_weights(case, name):
 WINDOWS = [  # nb, bt, kvh, gqa, d, bits, group, queries
     (3, 128, 2, 4, 128, 4, 32, 32), (3, 128, 2, 4, 128, 2, 32, 32), (7, 40, 1, 12, 64, 4, 64, 5),
     (5, 100, 3, 1, 96, 4, 32, 50), (5, 100, 2, 2, 96, 2, 96, 33), (9, 64, 2, 8, 128, 4, 128, 40),
-    (40, 17, 1, 3, 64, 2, 32, 64), (1, 1, 1, 33, 128, 4, 32, 1), (2, 300, 1, 129, 64, 4, 32, 2)]
+    (40, 17, 1, 3, 64, 2, 32, 64), (1, 1, 1, 33, 128, 4, 32, 1), (2, 300, 1, 129, 64, 4, 32, 2),
+    (2, 128, 2, 4, 256, 4, 64, 40), (3, 70, 1, 4, 256, 2, 32, 63), (2, 128, 1, 4, 256, 2, 256, 10),
+    (2, 100, 2, 4, 128, 4, 16, 30), (2, 100, 1, 5, 96, 2, 48, 11), (3, 30, 1, 40, 256, 4, 16, 1),
+    (2, 64, 2, 40, 64, 2, 16, 1), (5, 8, 1, 50, 96, 4, 16, 3)]
 
 
 @pytest.mark.parametrize("name", ["f32", "f16", "bf16", "f64"])
