@@ -8,6 +8,11 @@
 // two), and the accumulator starts at -8 2^-24 sum q, which is constant. The MMAs' FP32 sums then
 // round at the size of that start, which is the size of the codes' own sum. INT2 codes are mostly
 // zero, their sums far below such a start, so they are centred first (half as many bytes to unpack).
+//
+// One step of 8 KV heads x 4 query heads x 128: 131072 tokens INT4 20.8 us, 0.61 of the measured copy
+// rate (84 MB; about 5 us are the start, the rest runs at 0.77 of that rate, bound by issuing about
+// 310 instructions a 32-place tile); INT2 23.2 us; 8192 tokens 5.5 us, all of it start. Tiles of 16
+// places with three or four CTAs an SM took 28 to 36 us.
 #pragma once
 
 #include "weights_tc.cuh"
@@ -155,7 +160,7 @@ __global__ void __launch_bounds__(kThreads, step_resident(D, LO)) weights_step_k
     float l2 = INFINITY;  // lane i: of row i
     int see = 0;
     if (lane < j.rows) {
-      see = a.visible ? a.visible[lane / gqa] : 0x7fffffff;
+      see = a.visible ? max(a.visible[lane / gqa], 0) : 0x7fffffff;
       if (!j.parts)
         l2 = as_log2(a.lse_in[static_cast<long long>(lane / gqa) * a.qh + h * gqa + lane % gqa]);
     }

@@ -6,9 +6,9 @@
 // (FP32 and FP64 ones as a high and a low part), each row scaled by a power of two to the top of
 // FP16's range, so that every product is exact and the FP32 sums are the only rounding; the FP16 key
 // scales are constant over a unit of 32 (or 16) dims and multiply the unit's partial sums in FP32.
-// tcgen05 would need the dequantized FP16 keys in shared memory and a scale per row and unit between
-// its MMAs (none of its block scalings is FP16 per 16 or 32 elements), and at one decode step's 4 to
-// 8 query rows a unit the tensor work is a tenth of the copies' time.
+// More than 32 rows go to tcgen05 (weights_umma.cuh): its tiles are 128 rows wide however few are used.
+// 65536 tokens x 8 heads x 128 INT4, log-sum-exps computed: 16 rows 54 us and 32 rows 70 us here, 64 rows
+// 99 us and 128 rows 112 us there.
 //
 // Unit layout. A lane (r, c) of the A fragment holds the codes of row r (and r + 8) that lie c-th of
 // four in the unit: 8 codes of a 32-dim unit, 4 of a 16-dim unit, unpacked two at a time into pairs
@@ -151,6 +151,13 @@ __device__ __forceinline__ RowScales<UNITS> spread(const RowScales<UNITS>& g, in
   return spread_by<UNITS, 16>(g);  // one group: 6 or 16 units
 }
 
+// Whether query t of query head `head` adds to any place. One that sees nothing, or whose given
+// log-sum-exp says so, may hold anything (padding): it enters the products as zeros.
+__device__ __forceinline__ bool adds(const WeightsArgs& a, int t, int head) {
+  return !(a.visible && a.visible[t] <= 0) &&
+         !(a.lse_in && a.lse_in[static_cast<long long>(t) * a.qh + head] == -INFINITY);
+}
+
 // The B fragments of 8 query rows (lane: row lane / 4) and the factor that turns their sums into
 // scores in the log2 domain: sm_scale log2(e) / 2^e, with 2^e the row's scale.
 template <int D, int UNIT, bool LO>
@@ -167,6 +174,7 @@ struct QueryTile {
     float top = 0.f;
     if (row < j.rows) {
       const long long at = (static_cast<long long>(row / gqa) * a.qh + h * gqa + row % gqa) * D;
+      const bool live = adds(a, row / gqa, h * gqa + row % gqa);
 #pragma unroll
       for (int u = 0; u < kUnits; ++u) {
         if constexpr (kOwn == 8) {
@@ -176,7 +184,10 @@ struct QueryTile {
           for (int i = 0; i < kOwn; ++i) q[u][i] = load_query(a.query, a.dtype, at + u * UNIT + c * kOwn + i);
         }
 #pragma unroll
-        for (int i = 0; i < kOwn; ++i) top = fmaxf(top, fabsf(q[u][i]));
+        for (int i = 0; i < kOwn; ++i) {
+          if (!live) q[u][i] = 0.f;
+          top = fmaxf(top, fabsf(q[u][i]));
+        }
       }
     } else {
 #pragma unroll

@@ -478,6 +478,28 @@ def test_weights_masks_and_odd_values(geometry):
     check_weights(query * 0, kp, ks, valid, bits, group, 0.1, got=zero)
 
 
+@pytest.mark.parametrize("geometry", [(2, 2, 128, 4, 32, 4), (6, 4, 128, 4, 32, 4), (12, 4, 64, 2, 32, 4),
+                                      (6, 2, 32, 4, 8, 4), (12, 4, 256, 4, 64, 1), (2, 3, 96, 2, 16, 1)])
+def test_weights_padding_queries_may_hold_anything(geometry):
+    """Queries that see nothing, beside ones that see all, are NaN and infinite: nothing of them shows."""
+    queries, gqa, d, bits, group, kvh = geometry
+    kp, ks = key_pool(5, 64, kvh, d, bits, group, 12)
+    valid = torch.full((5,), 64, dtype=torch.int32, device=DEV)
+    clean = torch.randn(queries, kvh * gqa, d, generator=gen(2)).half().to(DEV)
+    visible = torch.full((queries,), 10**6, dtype=torch.int32, device=DEV)
+    visible[1::3], visible[2::3] = 0, -2**31
+    padded = clean.clone()
+    padded[1::3], padded[2::3] = math.nan, math.inf
+    want = ops.attention_weights(clean, kp, ks, valid, bits, group, 0.1, visible=visible)
+    check_weights(clean, kp, ks, valid, bits, group, 0.1, visible=visible, got=want)
+    got = ops.attention_weights(padded, kp, ks, valid, bits, group, 0.1, visible=visible)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    for seen in (visible, None):  # None: the -inf log-sum-exps alone tell
+        # the log-sum-exp goes through natural units: three roundings at its size, below 16
+        w, _ = ops.attention_weights(padded, kp, ks, valid, bits, group, 0.1, visible=seen, lse=want[1])
+        torch.testing.assert_close(w, want[0], rtol=1e-5, atol=0)
+
+
 @pytest.mark.parametrize("scale", [1e-6, 1.0, 3e4])
 def test_weights_query_ranges(scale):
     """FP32 and BF16 queries far outside FP16's range, with elements of very different size."""
