@@ -6,6 +6,10 @@
 // The angle is taken in FP64 and reduced to a fraction of a turn there (at a position of 10^6 an
 // FP32 angle is off by 0.03 rad); cos and sin of the reduced angle, the products and their sum are
 // FP32, rounded once to the element type.
+//
+// 8192 x 32 x 128 BF16: 22.7 us, 5.9 TB/s (0.90 of the measured copy rate), two batches a thread; with one
+// 24.0 us. With arrays of 16-bit elements in place of 32-bit words it took 40.6 us, and with divisions
+// in the loop 49.5.
 #include "cache_ops.cuh"
 
 namespace kvb {

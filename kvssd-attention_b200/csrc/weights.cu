@@ -6,7 +6,8 @@
 // first pass over the keys computes them.
 //
 // head_dim 64, 96, 128 and 256 with scale groups of whole 16 dims and aligned codes run on the
-// tensor cores (weights_tc.cuh). weights_lse_kernel, weights_combine_kernel and weights_kernel are the
+// tensor cores: up to 8 query rows a KV head by weights_step.cuh, up to 32 by weights_window.cuh, more by
+// weights_umma.cuh. weights_lse_kernel, weights_combine_kernel and weights_kernel are the
 // form for any other shape: a CTA takes one KV head and kPlaces places, a warp one place at a time,
 // the lanes the head's dims.
 #include "weights_tc.cuh"
