@@ -16,7 +16,7 @@
 //
 // A CTA walks a run of tiles: it waits for the MMAs of tile i, unpacks tile i + 1 into the one key buffer,
 // issues its MMAs into the other half of the accumulator, and works on tile i's scores while they run. Two
-// CTAs share an SM (one at head_dim 256). Codes are loaded a tile ahead into registers.
+// CTAs share an SM (one of twice the threads at head_dim 256). Codes are loaded a tile ahead into registers.
 //
 // 65536 tokens x 8 heads x 128 INT2, 32 queries x 4 query heads, both passes: 86 us, of which 30 are
 // exponentials; a tile takes a CTA about 3700 clocks (log-sum-exps) and 5100 (weights), unpacking and the
@@ -34,7 +34,6 @@ using weights_tc::kLn2;
 using weights_tc::kLog2e;
 using weights_tc::kLowest;
 
-constexpr int kThreads = 256;
 constexpr int kTile = 128;              // places, and query rows, of a tile
 constexpr int kBlockBytes = kTile * 128;  // 128 rows of 64 FP16: one swizzled block
 constexpr uint32_t kColumns = 256;      // TMEM: two accumulators of 128 columns
@@ -126,29 +125,35 @@ __device__ __forceinline__ void store_chunk(uint32_t at, uint32_t a, uint32_t b,
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
+// Threads of a place, or query row: warps w, w + 4, ... share the accumulator lanes of quarter w. Four where
+// one CTA has the SM (head_dim 256, 252 rows x 23561 places INT2: 51.0 us, two 71.5); with two CTAs an SM
+// two are faster (head_dim 128, 128 rows x 65536 places x 8 heads INT2: 86 us, four 103).
+constexpr int shares(int d) { return d <= 128 ? 2 : 4; }
+constexpr int threads(int d) { return 128 * shares(d); }
 constexpr int resident(int d) { return d <= 128 ? 2 : 1; }  // CTAs on an SM
 
 template <int BITS, int D, bool LO, bool LSE>
-__global__ void __launch_bounds__(kThreads, resident(D)) weights_umma_kernel(const Job j, Divisor bt_by) {
+__global__ void __launch_bounds__(threads(D), resident(D)) weights_umma_kernel(const Job j, Divisor bt_by) {
+  constexpr int kThreads = threads(D), kShares = shares(D), kChunks = 4 / kShares;  // 32-column chunks a share
   constexpr int kBlocks = (D + 63) / 64;        // swizzled blocks of a tile's row of FP16
   constexpr int kKeyTerms = BITS == 4 ? 2 : 1, kQueryTerms = LO ? 2 : 1;
   constexpr int kPieces = D / 32;               // 32-dim pieces of a row
-  constexpr int kOwn = (kPieces + 1) / 2;       // of them, a thread's: the first ones or the rest
+  constexpr int kOwn = (kPieces + kShares - 1) / kShares;  // of them, a thread's
   constexpr int kWords = BITS;                  // 32-bit words of codes of a piece
-  // both halves have whole pairs of pieces: their rows start on 16 bytes of INT2 codes, 4 of scales
-  constexpr bool kEven = kPieces % 4 == 0;
+  // all shares have whole pairs of pieces: they start on 16 bytes of INT2 codes, 4 of scales
+  constexpr bool kEven = kPieces % (2 * kShares) == 0;
   extern __shared__ uint8_t raw_smem[];
   __shared__ uint64_t done_bar;
   __shared__ uint32_t tmem_at;
   __shared__ int gave_up;
   __shared__ alignas(16) float4 infos[kTile / 2];  // of two rows: factors, negated log-sum-exps
   __shared__ alignas(16) int seen[kTile];
-  __shared__ float halves[2][kTile];
-  __shared__ float2 state[kTile];
+  __shared__ float sums_of[2][kShares - 1][kTile];
+  __shared__ float2 state[kShares - 1][kTile];
   __shared__ int2 slots[kMostSlots];  // (pool block, valid rows) of the run's selected blocks
   __shared__ uint32_t valid_mask[4][4];  // of tile i: [i & 3] (a warp may be a tile behind another)
   const WeightsArgs& a = j.a;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quarter = warp & 3, half = warp >> 2;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quarter = warp & 3, share = warp >> 2;
   const int row = quarter * 32 + lane;          // the place this thread unpacks; its accumulator lane
   const int h = blockIdx.y, gqa = a.qh / a.kvh, groups = D / a.group;
   const uint32_t base = (smem_addr(raw_smem) + 1023u) & ~1023u;
@@ -188,7 +193,7 @@ __global__ void __launch_bounds__(kThreads, resident(D)) weights_umma_kernel(con
     const int2 info = slots[slot - first_slot];
     const int blk = info.x;
     valid = in_block < info.y;
-    if (!LSE && half == 0 && (a.previous || j.add))
+    if (!LSE && share == 0 && (a.previous || j.add))
       prev = j.add ? a.out[h * a.out_stride + place] : a.previous[h * a.previous_stride + place];
     if (!valid) return;
     const long long r = (static_cast<long long>(blk) * a.bt + in_block) * a.kvh + h;
@@ -197,13 +202,13 @@ __global__ void __launch_bounds__(kThreads, resident(D)) weights_umma_kernel(con
     if constexpr (BITS == 2 && kEven) {  // two pieces in one access
 #pragma unroll
       for (int k = 0; k < kOwn; k += 2) {
-        const uint4 v = *reinterpret_cast<const uint4*>(from + (half * kOwn + k) * 8);
+        const uint4 v = *reinterpret_cast<const uint4*>(from + (share * kOwn + k) * 8);
         code[k][0] = v.x, code[k][1] = v.y, code[k + 1][0] = v.z, code[k + 1][1] = v.w;
       }
     } else {
 #pragma unroll
       for (int k = 0; k < kOwn; ++k) {
-        const int piece = half * kOwn + k;
+        const int piece = share * kOwn + k;
         if (piece >= kPieces) continue;
         if constexpr (BITS == 4) {
           const uint4 v = *reinterpret_cast<const uint4*>(from + piece * 16);
@@ -217,11 +222,11 @@ __global__ void __launch_bounds__(kThreads, resident(D)) weights_umma_kernel(con
     const unsigned short* u = reinterpret_cast<const unsigned short*>(s);
     if (in_pairs) {
 #pragma unroll
-      for (int k = 0; k < kOwn; k += 2) scale[k] = *reinterpret_cast<const uint32_t*>(u + half * kOwn + k);
+      for (int k = 0; k < kOwn; k += 2) scale[k] = *reinterpret_cast<const uint32_t*>(u + share * kOwn + k);
     } else {
 #pragma unroll
       for (int k = 0; k < kOwn; ++k) {
-        const int piece = min(half * kOwn + k, kPieces - 1);
+        const int piece = min(share * kOwn + k, kPieces - 1);
         if (a.group == 16) scale[k] = reinterpret_cast<const uint32_t*>(u)[piece];
         else if (in_halves) scale[k] = u[32 * piece / a.group] | static_cast<uint32_t>(u[(32 * piece + 16) / a.group]) << 16;
         else scale[k] = u[32 * piece / a.group];
@@ -235,7 +240,7 @@ __global__ void __launch_bounds__(kThreads, resident(D)) weights_umma_kernel(con
     if (!valid) return large;
 #pragma unroll
     for (int k = 0; k < kOwn; ++k) {
-      const int piece = half * kOwn + k;
+      const int piece = share * kOwn + k;
       if (piece >= kPieces) continue;
       constexpr uint32_t kLimit = BITS == 4 ? 0x6FFFu : 0x77FFu;
       const uint32_t one = in_pairs ? scale[k & ~1] >> (16 * (k & 1)) & 0xFFFFu : scale[k];
@@ -288,10 +293,10 @@ __global__ void __launch_bounds__(kThreads, resident(D)) weights_umma_kernel(con
   }
   load(0);
 
-  // ---- the query rows: two threads a row, taking turns at its units of 16 dims; their infos
+  // ---- the query rows: kShares threads a row, taking turns at its units of 16 dims; their infos
   {
-    constexpr int kUnits = D / 16, kMine = (kUnits + 1) / 2;
-    const int r = threadIdx.x >> 1, side = threadIdx.x & 1, at = row0 + r;
+    constexpr int kUnits = D / 16, kMine = (kUnits + kShares - 1) / kShares;
+    const int r = threadIdx.x / kShares, side = threadIdx.x % kShares, at = row0 + r;
     const bool live = r < rows;
     const int t = live ? at / gqa : 0, head = h * gqa + (live ? at % gqa : 0);
     const long long q = (static_cast<long long>(t) * a.qh + head) * D;
@@ -299,7 +304,7 @@ __global__ void __launch_bounds__(kThreads, resident(D)) weights_umma_kernel(con
     float top = 0.f;
 #pragma unroll
     for (int k = 0; k < kMine; ++k) {
-      const int unit = side + 2 * k;
+      const int unit = side + kShares * k;
       if (!live || unit >= kUnits) continue;
       load_query8(a.query, a.dtype, q + 16 * unit, x[k][0]);
       load_query8(a.query, a.dtype, q + 16 * unit + 8, x[k][1]);
@@ -312,7 +317,8 @@ __global__ void __launch_bounds__(kThreads, resident(D)) weights_umma_kernel(con
         if (!enters) x[k][i >> 3][i & 7] = 0.f;
         top = fmaxf(top, fabsf(x[k][i >> 3][i & 7]));
       }
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+#pragma unroll
+    for (int o = 1; o < kShares; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     int e = 0;
     if (top > 0.f && top < INFINITY) e = 14 - ilogbf(top);
     const auto power = [](int i) { return __int_as_float((i + 127) << 23); };
@@ -322,7 +328,7 @@ __global__ void __launch_bounds__(kThreads, resident(D)) weights_umma_kernel(con
     const float factor = fabsf(a.sm_scale) * kLog2e * power(-e1) * power(-e2);
 #pragma unroll
     for (int k = 0; k < kMine; ++k) {
-      const int unit = side + 2 * k;
+      const int unit = side + kShares * k;
       if (unit >= kUnits) continue;
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
@@ -350,16 +356,20 @@ __global__ void __launch_bounds__(kThreads, resident(D)) weights_umma_kernel(con
                              (static_cast<long long>(h) * j.rows + (live ? at : 0)) * j.parts;
         float m = kLowest, l = 0.f;
 #pragma unroll 8
-        for (int p = 0; p < j.parts; p += 2) {
+        for (int p = 0; p < j.parts; p += kShares) {
           const float2 v = p + side < j.parts ? part[p + side] : make_float2(kLowest, 0.f);
           const float up = fmaxf(m, v.x);
           l = l * fast_exp2(m - up) + v.y * fast_exp2(v.x - up);
           m = up;
         }
-        const float m2 = __shfl_xor_sync(0xffffffffu, m, 1), l3 = __shfl_xor_sync(0xffffffffu, l, 1);
-        const float up = fmaxf(m, m2);
-        l = l * fast_exp2(m - up) + l3 * fast_exp2(m2 - up);
-        l2 = l == 0.f ? -INFINITY : up + log2f(l);
+#pragma unroll
+        for (int o = 1; o < kShares; o <<= 1) {
+          const float m2 = __shfl_xor_sync(0xffffffffu, m, o), l3 = __shfl_xor_sync(0xffffffffu, l, o);
+          const float up = fmaxf(m, m2);
+          l = l * fast_exp2(m - up) + l3 * fast_exp2(m2 - up);
+          m = up;
+        }
+        l2 = l == 0.f ? -INFINITY : m + log2f(l);
         if (live && blockIdx.x == 0 && side == 0) a.lse[to] = l2 * kLn2;
         if (l2 == -INFINITY) l2 = INFINITY;
       } else if (live) {
@@ -408,7 +418,7 @@ __global__ void __launch_bounds__(kThreads, resident(D)) weights_umma_kernel(con
       large = unpack(kOne);
       mine_prev = prev;
       const uint32_t mask = __ballot_sync(0xffffffffu, valid);
-      if (half == 0 && lane == 0) valid_mask[i & 3][quarter] = mask;
+      if (share == 0 && lane == 0) valid_mask[i & 3][quarter] = mask;
     }
     fence_async_proxy();
     fence_before_sync();
@@ -436,8 +446,17 @@ __global__ void __launch_bounds__(kThreads, resident(D)) weights_umma_kernel(con
   const float own_factor = reinterpret_cast<const float*>(infos + row / 2)[row & 1];
   const int own_seen = seen[row];
   const uint32_t lanes_at = static_cast<uint32_t>(quarter * 32) << 16;
-  float run_m = kLowest, run_l = 0.f;  // LSE: of query row `row` over this half of the columns
-  float sum = 0.f, sum_prev = 0.f;     // weights: of the last tile's place `row`, this half
+  float run_m = kLowest, run_l = 0.f;  // LSE: of query row `row` over this share of the columns
+  float sum = 0.f, sum_prev = 0.f;     // weights: of the last tile's place `row`, this share
+
+  const auto write = [&](int i) {
+    const int place = (first_tile + i) * kTile + row;
+    if (place >= places) return;
+    float all = sum;
+#pragma unroll
+    for (int k = 0; k < kShares - 1; ++k) all += sums_of[i & 1][k][row];
+    a.out[h * a.out_stride + place] = sum_prev + all;
+  };
 
   int i = 0;
   for (; i < tiles; ++i) {
@@ -449,27 +468,27 @@ __global__ void __launch_bounds__(kThreads, resident(D)) weights_umma_kernel(con
     next_valid = mine_valid;
     next_prev = mine_prev;
     if (stop) break;  // all threads
-    if (!LSE && half == 0 && i > 0) {  // the other half of the last tile's columns has arrived
-      const int place = (first_tile + i - 1) * kTile + row;
-      if (place < places) a.out[h * a.out_stride + place] = sum_prev + (sum + halves[i - 1 & 1][row]);
-    }
+    if (!LSE && share == 0 && i > 0) write(i - 1);  // the other shares' sums have arrived
     load(i + 2);
 
     const int place0 = (first_tile + i) * kTile;
     const uint32_t acc = tmem_at + (i & 1) * kTile + lanes_at;
     if constexpr (LSE) {
-      const uint32_t* mask = valid_mask[i & 3] + 2 * half;
-      const bool full = (mask[0] & mask[1]) == 0xFFFFFFFFu && place0 + kTile <= all_see;
-      const float scaled = large ? own_factor * 16.f : own_factor;
-      float both[2][32];
-      tmem_load32(acc + half * 64, both[0]);
+      const uint32_t* mask = valid_mask[i & 3] + kChunks * share;
+      bool full = place0 + kTile <= all_see;
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        float (&v)[32] = both[c];
+      for (int c = 0; c < kChunks; ++c) full = full && mask[c] == 0xFFFFFFFFu;
+      const float scaled = large ? own_factor * 16.f : own_factor;
+      const int column0 = share * 32 * kChunks;
+      float chunks[kChunks][32];
+      tmem_load32(acc + column0, chunks[0]);
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) {
+        float (&v)[32] = chunks[c];
         tmem_wait(v);
-        if (c == 0) tmem_load32(acc + half * 64 + 32, both[1]);  // while these are worked on
+        if (c + 1 < kChunks) tmem_load32(acc + column0 + 32 * (c + 1), chunks[(c + 1) % kChunks]);  // while these are worked on
         if (!full) {
-          const int see = own_seen - (place0 + half * 64 + c * 32);  // columns seen
+          const int see = own_seen - (place0 + column0 + c * 32);  // columns seen
           const uint32_t live = mask[c] & (see <= 0 ? 0u : see >= 32 ? 0xFFFFFFFFu : (1u << see) - 1u);
 #pragma unroll
           for (int k = 0; k < 32; ++k) v[k] = live >> k & 1u ? v[k] * scaled : -INFINITY;
@@ -490,22 +509,22 @@ __global__ void __launch_bounds__(kThreads, resident(D)) weights_umma_kernel(con
           const float2 x = parts(fma2(f2(v[k], v[k + 1]), by, less));
           part[k / 2 & 1] = add2(part[k / 2 & 1], f2(fast_exp2(x.x), fast_exp2(x.y)));
         }
-        const float2 both_sums = parts(add2(part[0], part[1]));
-        run_l += both_sums.x + both_sums.y;
+        const float2 sums = parts(add2(part[0], part[1]));
+        run_l += sums.x + sums.y;
       }
     } else {
       const bool full = place0 + kTile <= all_see;
       F2 part[2] = {f2(0.f), f2(0.f)};
-      // the columns' chunks of 32 alternate between the halves
-      float both[2][32];
-      if (half * 32 < columns) tmem_load32(acc + half * 32, both[0]);
+      // the columns' chunks of 32 alternate between the shares
+      float chunks[kChunks][32];
+      if (share * 32 < columns) tmem_load32(acc + share * 32, chunks[0]);
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const int c = half * 32 + n * 64;
+      for (int n = 0; n < kChunks; ++n) {
+        const int c = (share + n * kShares) * 32, next = c + kShares * 32;
         if (c >= columns) break;
-        float (&v)[32] = both[n];
+        float (&v)[32] = chunks[n];
         tmem_wait(v);
-        if (n == 0 && c + 64 < columns) tmem_load32(acc + c + 64, both[1]);  // while these are worked on
+        if (n + 1 < kChunks && next < columns) tmem_load32(acc + next, chunks[(n + 1) % kChunks]);  // while these are worked on
         if (large) {
 #pragma unroll
           for (int k = 0; k < 32; ++k) v[k] *= 16.f;
@@ -526,7 +545,7 @@ __global__ void __launch_bounds__(kThreads, resident(D)) weights_umma_kernel(con
       const float2 sums = parts(add2(part[0], part[1]));
       sum = place_valid ? sums.x + sums.y : 0.f;
       sum_prev = place_prev;
-      if (half == 1) halves[i & 1][row] = sum;
+      if (share > 0) sums_of[i & 1][share - 1][row] = sum;
     }
   }
 
@@ -535,7 +554,7 @@ __global__ void __launch_bounds__(kThreads, resident(D)) weights_umma_kernel(con
     wait_done(bar, i & 1);
     const float nan = __int_as_float(0x7fffffff);
     run_l = run_m = nan;
-    if (!LSE && half == 0)
+    if (!LSE && share == 0)
       for (int t = max(i - 1, 0); t < tiles; ++t) {
         const int place = (first_tile + t) * kTile + row;
         if (place < places) a.out[h * a.out_stride + place] = nan;
@@ -544,20 +563,23 @@ __global__ void __launch_bounds__(kThreads, resident(D)) weights_umma_kernel(con
   fence_before_sync();
   __syncthreads();
   if constexpr (LSE) {
-    if (half == 1) state[row] = make_float2(run_m, run_l);
+    if (share > 0) state[share - 1][row] = make_float2(run_m, run_l);
     __syncthreads();
-    if (half == 0 && row < rows) {
-      const float2 other = state[row];
-      const float top = fmaxf(run_m, other.x);
-      float2 part = make_float2(top, run_l * fast_exp2(run_m - top) + other.y * fast_exp2(other.x - top));
+    if (share == 0 && row < rows) {
+      float2 part = make_float2(run_m, run_l);
+#pragma unroll
+      for (int k = 0; k < kShares - 1; ++k) {
+        const float2 other = state[k][row];
+        const float top = fmaxf(part.x, other.x);
+        part = make_float2(top, part.y * fast_exp2(part.x - top) + other.y * fast_exp2(other.x - top));
+      }
       if (own_seen <= 0) part = make_float2(kLowest, 0.f);
       if (stop) part = make_float2(0.f, __int_as_float(0x7fffffff));
       reinterpret_cast<float2*>(a.scratch)[(static_cast<long long>(h) * j.rows + row0 + row) * j.parts +
                                            blockIdx.x] = part;
     }
-  } else if (half == 0 && !stop) {
-    const int place = (first_tile + tiles - 1) * kTile + row;
-    if (place < places) a.out[h * a.out_stride + place] = sum_prev + (sum + halves[tiles - 1 & 1][row]);
+  } else if (share == 0 && !stop) {
+    write(tiles - 1);
   }
   if (warp == 0) tmem_free(tmem_at);
 }
@@ -582,7 +604,7 @@ cudaError_t launch_pass(Job j, cudaStream_t s) {
   const int z = LSE && chunks <= 65535 ? chunks : 1;
   for (j.row0 = 0; j.row0 < j.rows; j.row0 += z * kTile) {
     j.add = j.row0 > 0;
-    const cudaError_t l = launch_pdl(kernel, dim3(ctas, j.a.kvh, z), kThreads, smem, s, j,
+    const cudaError_t l = launch_pdl(kernel, dim3(ctas, j.a.kvh, z), threads(D), smem, s, j,
                                      divisor(static_cast<unsigned>(j.a.bt)));
     if (l != cudaSuccess) return l;
   }
