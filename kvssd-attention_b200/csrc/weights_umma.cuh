@@ -300,6 +300,8 @@ __global__ void __launch_bounds__(threads(D), resident(D)) weights_umma_kernel(c
     const bool live = r < rows;
     const int t = live ? at / gqa : 0, head = h * gqa + (live ? at % gqa : 0);
     const long long q = (static_cast<long long>(t) * a.qh + head) * D;
+    const int n = !live ? 0 : a.visible ? a.visible[t] : 0x7fffffff;
+    const float given = a.lse_in && live ? a.lse_in[static_cast<long long>(t) * a.qh + head] : 0.f;
     float x[kMine][2][8] = {};
     float top = 0.f;
 #pragma unroll
@@ -309,7 +311,8 @@ __global__ void __launch_bounds__(threads(D), resident(D)) weights_umma_kernel(c
       load_query8(a.query, a.dtype, q + 16 * unit, x[k][0]);
       load_query8(a.query, a.dtype, q + 16 * unit + 8, x[k][1]);
     }
-    const bool enters = live && weights_tc::adds(a, t, head);
+    // a row that adds nothing may hold anything (padding): it enters the products as zeros
+    const bool enters = n > 0 && given != -INFINITY;
 #pragma unroll
     for (int k = 0; k < kMine; ++k)
 #pragma unroll
@@ -347,7 +350,6 @@ __global__ void __launch_bounds__(threads(D), resident(D)) weights_umma_kernel(c
         if constexpr (LO) store_chunk(to + kBlocks * kBlockBytes, lo[0], lo[1], lo[2], lo[3]);
       }
     }
-    const int n = !live ? 0 : a.visible ? a.visible[t] : 0x7fffffff;
     float l2 = LSE ? 0.f : INFINITY;
     if constexpr (!LSE) {
       const long long to = static_cast<long long>(t) * a.qh + head;
@@ -373,7 +375,7 @@ __global__ void __launch_bounds__(threads(D), resident(D)) weights_umma_kernel(c
         if (live && blockIdx.x == 0 && side == 0) a.lse[to] = l2 * kLn2;
         if (l2 == -INFINITY) l2 = INFINITY;
       } else if (live) {
-        l2 = as_log2(a.lse_in[to]);
+        l2 = as_log2(given);
       }
       if (n <= 0) l2 = INFINITY;
     }
