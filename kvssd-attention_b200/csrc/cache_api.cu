@@ -84,6 +84,8 @@ int kvssd_b200_append(const void* key, const void* value, int dtype, long long k
                       int head_dim, int bits, int group_size, uint16_t* key_values,
                       uint16_t* value_values, unsigned* device_status, kvssd_b200_stream_t stream) {
   if (tokens < 0) return bad("tokens must not be negative");
+  if (tokens > 0x7ff00000)  // room for a CTA's tokens behind the last
+    return report(KVSSD_B200_ERR_UNSUPPORTED, "more than 2^31 tokens are not supported");
   if (int st = check_elements(dtype)) return st;
   if (int st = check_cache(n_pool_blocks, block_tokens, kv_heads, head_dim, bits, group_size)) return st;
   if (frequencies)

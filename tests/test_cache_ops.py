@@ -67,6 +67,10 @@ def test_append_unsupported_and_empty():
     assert _append(tokens=0, k=None) == 0
 
 
+def test_append_of_too_many_tokens():
+    _refused(_append(tokens=2**31 - 1), b"2^31", _native.ERR_UNSUPPORTED)
+
+
 def _weights(**kw):
     a = dict(q=DUMMY, dtype=1, queries=1, pk=DUMMY, sk=DUMMY, valid=DUMMY, table=None, visible=None,
              n_pool=2, n_sel=2, bt=8, qh=4, kvh=2, d=64, bits=4, group=32, scale=0.125, given=1,
