@@ -230,44 +230,49 @@ struct alignas(16) Eight {
   }
 };
 
-// A lane holds 8 consecutive elements of a row (head), a row is d / 8 lanes, a warp 32 / (d / 8) rows at
-// a time; a task is kIters such steps over the heads of one token's keys or values, their loads all in
-// flight at once. The cos and sin of the token's pairs are computed by the task's lanes and handed
-// around through shared memory, then stay in registers over the heads; a rotation's other element comes
-// from a lane of the same row (half layout) or is the lane's own (interleaved). kGroupLanes: the lanes
-// of a scale group, 0: any number of them.
+// A lane holds 8 consecutive elements of a row (head), a row is d / 8 lanes, a warp takes `heads` rows at a
+// time; a task is kIters such steps over the heads of one token's keys or values, their loads all in flight
+// at once. Where one step takes all heads and leaves half of a warp's lanes or more without work, a task is
+// that step of `per_warp` tokens (8.4 M elements, one head of 64: 63 us, with one token a warp 244). The cos
+// and sin of a token's pairs are computed by the task's lanes and handed around through shared memory, then
+// stay in registers over the heads; a rotation's other element comes from a lane of the same row (half
+// layout) or is the lane's own (interleaved). kGroupLanes: the lanes of a scale group, 0: any number.
 // TURNS: whether a task's keys may be rotated; the kernel without it needs half the registers.
 constexpr int resident(int iters, int bytes, bool turns) {
-  return turns ? (iters == 4 && bytes == 2 ? 3 : 2) : (bytes == 2 ? 4 : 3);
+  return turns ? (bytes == 2 ? 3 : 2) : (bytes == 2 ? 4 : 3);
 }
 
 template <typename T, int BITS, bool INTERLEAVED, int kIters, int kGroupLanes, bool TURNS>
 __global__ void __launch_bounds__(kThreads, resident(kIters, sizeof(T), TURNS))
-    append_rows_kernel(const AppendArgs a, int chunks, unsigned per_lane, int kv0) {
-  extern __shared__ Turn turns[];  // [warps][pairs]
+    append_rows_kernel(const AppendArgs a, int chunks, unsigned per_lane, int heads, int per_warp, int kv0) {
+  extern __shared__ Turn turns[];  // [warps][per_warp][pairs]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int lanes = a.d >> 3;                                   // of a row
-  const int rows = 32u * per_lane >> 16, row = lane * per_lane >> 16;  // of a warp; this lane's
+  const int row = lane * per_lane >> 16;  // of the warp
   const int l = lane - row * lanes;
+  const int step = kIters == 1 ? heads : 32u * per_lane >> 16;  // several steps use all of a warp's rows
+  const int tokens = kIters == 1 ? per_warp : 1;  // of the warp
+  const int nth = kIters == 1 ? row / step : 0, step_row = row - nth * step;
   const int later = static_cast<int>(blockIdx.y) >= chunks, kv = kv0 + later, chunk = blockIdx.y - later * chunks;
-  const int token = blockIdx.x * (kThreads / 32) + warp;
+  const int token0 = (blockIdx.x * (kThreads / 32) + warp) * tokens, token = token0 + nth;
   const int pairs = a.freq ? a.pairs : 0;
   pdl_wait();
   pdl_launch();
-  if (token >= a.tokens) return;
+  if (token0 >= a.tokens) return;
+  const bool live = kIters == 1 ? nth < tokens && token < a.tokens : row < step;  // lanes with a row
 
   const RowTensor& in = kv ? a.value : a.key;
   const T* x = static_cast<const T*>(in.p) + token * in.token + l * 8;
   Eight<T> data[kIters];
-  const int head0 = chunk * rows * kIters + row;
+  const int head0 = chunk * step * kIters + step_row;
 #pragma unroll
   for (int i = 0; i < kIters; ++i) {
-    const int h = head0 + i * rows;
-    if (row < rows && h < a.kvh) data[i].load(x + h * in.head);
+    const int h = head0 + i * step;
+    if (live && h < a.kvh) data[i].load(x + h * in.head);
     else data[i] = {};
   }
-  const long long slot = pool_row(a, index_at(a.slots, token));
-  if (kv == 0 && chunk == 0 && lane == 0 && slot >= 0 && a.valid) {
+  const long long slot = live ? pool_row(a, index_at(a.slots, token)) : -1;
+  if (kv == 0 && chunk == 0 && step_row == 0 && l == 0 && slot >= 0 && a.valid) {
     // below 2^32 rows (nearly always) the division is the short one
     const long long block = slot >> 32 ? slot / a.bt : static_cast<unsigned>(slot) / static_cast<unsigned>(a.bt);
     atomicMax(a.valid + block, static_cast<int>(slot - block * a.bt) + 1);
@@ -279,26 +284,28 @@ __global__ void __launch_bounds__(kThreads, resident(kIters, sizeof(T), TURNS))
   int other = lane;  // the lane that holds the pairs' other elements: half layout
   const bool turning = TURNS && kv == 0 && pairs > 0;  // the same for the whole warp
   if (turning) {
-    Turn* mine = turns + warp * pairs;
-    const long long position = index_at(a.positions, token);
+    Turn* mine = turns + warp * tokens * pairs;
     // pair i at (i % kRun) * (pairs / kRun) + i / kRun: lanes read consecutive entries
     constexpr int kRun = INTERLEAVED ? 4 : 8;
-    const int step = pairs / kRun;
-    for (int i = lane; i < pairs; i += 32)
-      mine[i % kRun * step + i / kRun] = make_turn<T>(position, a.freq[i], a.magnitude);
+    const int runs = pairs / kRun;
+    for (int t = 0; t == 0 || (kIters == 1 && t < tokens && token0 + t < a.tokens); ++t) {
+      const long long position = index_at(a.positions, token0 + t);
+      for (int i = lane; i < pairs; i += 32)
+        mine[t * pairs + i % kRun * runs + i / kRun] = make_turn<T>(position, a.freq[i], a.magnitude);
+    }
     __syncwarp();
-    const bool rotated = row < rows && l * 8 < 2 * pairs, second = l * 8 >= pairs;
-    const Turn* own = mine + (INTERLEAVED || !second ? l : l - pairs / 8);
+    const bool rotated = live && l * 8 < 2 * pairs, second = l * 8 >= pairs;
+    const Turn* own = mine + nth * pairs + (INTERLEAVED || !second ? l : l - pairs / 8);
     const float sign = second ? 1.f : -1.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       ch[i] = f2(1.f), cl[i] = sh[i] = sl[i] = f2(0.f);
       if (!rotated) continue;
       if constexpr (INTERLEAVED) {
-        const Turn t = own[i * step];
+        const Turn t = own[i * runs];
         ch[i] = f2(t.ch), cl[i] = f2(t.cl), sh[i] = f2(-t.sh, t.sh), sl[i] = f2(-t.sl, t.sl);
       } else {
-        const Turn t = own[2 * i * step], u = own[(2 * i + 1) * step];
+        const Turn t = own[2 * i * runs], u = own[(2 * i + 1) * runs];
         ch[i] = f2(t.ch, u.ch), cl[i] = f2(t.cl, u.cl);
         sh[i] = f2(sign * t.sh, sign * u.sh), sl[i] = f2(sign * t.sl, sign * u.sl);
       }
@@ -317,7 +324,7 @@ __global__ void __launch_bounds__(kThreads, resident(kIters, sizeof(T), TURNS))
 #pragma unroll
   for (int i = 0; i < kIters; ++i) {
     // no early end: the iterations' chains of dependent operations overlap
-    const bool mine = row < rows && head0 + i * rows < a.kvh;
+    const bool mine = live && head0 + i * step < a.kvh;
     F2 v[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) v[k] = unpack_pair<T>(data[i].w, k);
@@ -359,48 +366,55 @@ __global__ void __launch_bounds__(kThreads, resident(kIters, sizeof(T), TURNS))
     F2 code[4];
     quantize8<BITS>(v, scale, code);
     const uint32_t bytes = pack8<BITS>(code);
-    uint8_t* to = codes + i * (rows * lanes * BITS);
+    uint8_t* to = codes + i * (step * lanes * BITS);
     if (mine && slot >= 0) {
       if constexpr (BITS == 4) *reinterpret_cast<uint32_t*>(to) = bytes;
       else *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(bytes);
     }
-    if (mine && slot >= 0 && leads) scales[i * (rows * groups)] = held;
+    if (mine && slot >= 0 && leads) scales[i * (step * groups)] = held;
     if (mine && values) {
       const F2 unit = f2(__half2float(held));
       uint32_t out[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) pack_pair<__half>(mul2(add2(code[k], f2(-kMid)), unit), out, k);
-      *reinterpret_cast<uint4*>(values + i * (rows * lanes * 8)) = make_uint4(out[0], out[1], out[2], out[3]);
+      *reinterpret_cast<uint4*>(values + i * (step * lanes * 8)) = make_uint4(out[0], out[1], out[2], out[3]);
     }
   }
 }
 
-template <typename T, int BITS, bool INTERLEAVED>
-cudaError_t launch_rows(const AppendArgs& a, cudaStream_t s) {
-  const int rows = 32 / (a.d / 8), warps = kThreads / 32;
-  // Four steps a task keep 2 KB a warp in flight; with few tokens one step a task spreads the work
-  // over more warps instead.
-  const int long_chunks = (a.kvh + 4 * rows - 1) / (4 * rows), short_chunks = (a.kvh + rows - 1) / rows;
-  const bool few = 2ll * a.tokens * long_chunks < 148 * 16;
-  const int chunks = few ? short_chunks : long_chunks;
+template <typename T, int BITS, bool INTERLEAVED, int kIters>
+cudaError_t launch_iters(const AppendArgs& a, int step, int per_warp, bool few, cudaStream_t s) {
+  const int warps = kThreads / 32, chunks = (a.kvh + kIters * step - 1) / (kIters * step);
   // lane / lanes as a product: 2^16 / lanes rounded up is exact for 32 lanes
   const unsigned per_lane = (65536u + a.d / 8 - 1) / (a.d / 8);
-  const dim3 both((a.tokens + warps - 1) / warps, 2 * chunks), one(both.x, chunks);
-  const size_t smem = a.freq ? static_cast<size_t>(warps) * a.pairs * sizeof(Turn) : 0;
+  const dim3 both((a.tokens + warps * per_warp - 1) / (warps * per_warp), 2 * chunks), one(both.x, chunks);
+  const size_t smem = a.freq ? static_cast<size_t>(warps) * per_warp * a.pairs * sizeof(Turn) : 0;
   const bool g32 = a.group == 32;
-  if (few)
-    return launch_pdl(g32 ? append_rows_kernel<T, BITS, INTERLEAVED, 1, 4, true>
-                          : append_rows_kernel<T, BITS, INTERLEAVED, 1, 0, true>,
-                      both, kThreads, smem, s, a, chunks, per_lane, 0);
+  const auto turned = g32 ? append_rows_kernel<T, BITS, INTERLEAVED, kIters, 4, true>
+                          : append_rows_kernel<T, BITS, INTERLEAVED, kIters, 0, true>;
+  if (few) return launch_pdl(turned, both, kThreads, smem, s, a, chunks, per_lane, step, per_warp, 0);
   // Many tokens: values (and keys that do not turn) in a launch of their own, which needs half the
   // registers (8192 tokens that do not turn: 14.8 us, by the kernel that can turn 18.5; keys that turn make
   // the two launches 26.8 us, in one 26.4).
-  const auto plain = g32 ? append_rows_kernel<T, BITS, false, 4, 4, false> : append_rows_kernel<T, BITS, false, 4, 0, false>;
-  const cudaError_t e = launch_pdl(plain, a.freq ? one : both, kThreads, 0, s, a, chunks, per_lane, a.freq ? 1 : 0);
+  const auto plain = g32 ? append_rows_kernel<T, BITS, false, kIters, 4, false>
+                         : append_rows_kernel<T, BITS, false, kIters, 0, false>;
+  const cudaError_t e = launch_pdl(plain, a.freq ? one : both, kThreads, 0, s, a, chunks, per_lane, step, per_warp,
+                                   a.freq ? 1 : 0);
   if (e != cudaSuccess || !a.freq) return e;
-  return launch_pdl(g32 ? append_rows_kernel<T, BITS, INTERLEAVED, 4, 4, true>
-                        : append_rows_kernel<T, BITS, INTERLEAVED, 4, 0, true>,
-                    one, kThreads, smem, s, a, chunks, per_lane, 0);
+  return launch_pdl(turned, one, kThreads, smem, s, a, chunks, per_lane, step, per_warp, 0);
+}
+
+template <typename T, int BITS, bool INTERLEAVED>
+cudaError_t launch_rows(const AppendArgs& a, cudaStream_t s) {
+  // Heads a warp takes at a time, and steps to take them all. Up to four steps a task keep 2 KB a warp in
+  // flight, no more than there are heads for (4 heads of 128: two steps 30.2 us, four 39.7); with few tokens
+  // one step a task spreads the work over more warps instead.
+  const int rows = 32 / (a.d / 8), step = rows < a.kvh ? rows : a.kvh, steps = (a.kvh + step - 1) / step;
+  const bool few = 2ll * a.tokens * ((steps + 3) / 4) < 148 * 16;
+  if (few) return launch_iters<T, BITS, INTERLEAVED, 1>(a, step, 1, true, s);
+  if (steps == 1) return launch_iters<T, BITS, INTERLEAVED, 1>(a, step, rows / step, false, s);
+  if (steps == 2) return launch_iters<T, BITS, INTERLEAVED, 2>(a, step, 1, false, s);
+  return launch_iters<T, BITS, INTERLEAVED, 4>(a, step, 1, false, s);
 }
 
 // Whether append_rows_kernel takes this call.

@@ -181,6 +181,19 @@ def test_append(case, interleaved, name):
     assert ops.read_device_status(DEV) == 0
 
 
+MANY = [  # so many tokens that a warp takes several of them, or two or four steps of heads
+    (2049, 1, 64, 4, 32, 40, 32), (1501, 1, 128, 2, 64, 64, 32), (1203, 2, 128, 4, 16, 128, 64),
+    (1301, 3, 96, 4, 32, 24, 48), (1999, 1, 16, 2, 8, 24, 8), (1250, 5, 40, 4, 8, 16, 16), (1250, 2, 24, 2, 24, 16, 8),
+    (1301, 4, 128, 2, 32, 64, 64), (1190, 2, 256, 4, 64, 32, 64), (1187, 7, 128, 4, 32, 64, 64), (2500, 1, 8, 4, 8, 64, 0)]
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("case", MANY)
+def test_append_many_tokens(case, interleaved, name):
+    test_append(case, interleaved, name)
+
+
 def test_append_strided_int32_and_without_values():
     pool, again = (make_pool(4, 16, 4, 128, 4, 32) for _ in range(2))
     g = gen(8)
