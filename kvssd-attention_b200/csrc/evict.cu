@@ -621,7 +621,7 @@ template <int E>
 cudaError_t select_in_registers(const EvictArgs& a, int ranks, int lists, int vectors, cudaStream_t s) {
   const auto kernel = evict_select_kernel<E>;
   constexpr size_t smem = sizeof(unsigned) * (kThreads * E + 2 * kDigits);
-  if (smem > 48 * 1024) {
+  if (smem >= 48 * 1024) {  // with the kernel's static shared memory more than is had unasked
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return e;
   }

@@ -735,6 +735,19 @@ def test_evict_long_caches_by_head(n, shared):
             np.testing.assert_array_equal(now[keep:], flat[keep:])
 
 
+@pytest.mark.parametrize("shared", [False, True])
+@pytest.mark.parametrize("n", [4095, 4097, 8193, 16385, 32768, 32769, 50_001, 65_537, 131_071, 131_073])
+def test_evict_lengths(n, shared):
+    """To either side of the lengths at which the selection takes more CTAs or more places a thread."""
+    test_evict_long_caches_by_head(n, shared)
+
+
+@pytest.mark.parametrize("n", [8192, 12_000, 16_385, 40_000])
+def test_evict_many_heads(n):
+    w, pos = stats(40, -(-n // 64) * 64, n, n)
+    check_evict(w, pos, n, n // 2, -(-n // 64), 64, 4, 1, recent=9)
+
+
 def test_evict_refuses_blocks_outside_the_pool():
     ops.read_device_status(DEV)
     w, pos = stats(1, 32, 32, 3)
