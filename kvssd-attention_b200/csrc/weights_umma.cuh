@@ -18,7 +18,7 @@
 // issues its MMAs into the other half of the accumulator, and works on tile i's scores while they run. Two
 // CTAs share an SM (one of twice the threads at head_dim 256). Codes are loaded a tile ahead into registers.
 //
-// 65536 tokens x 8 heads x 128 INT2, 32 queries x 4 query heads, both passes: 86 us, of which 30 are
+// 65536 tokens x 8 heads x 128 INT2, 32 queries x 4 query heads, both passes: 88 us, of which 30 are
 // exponentials; a tile takes a CTA about 3700 clocks (log-sum-exps) and 5100 (weights), unpacking and the
 // barriers' turns beside the exponentials, and a pass about 4.5 us to start. INT4: 112 us.
 #pragma once
