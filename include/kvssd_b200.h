@@ -423,7 +423,7 @@ KVSSD_B200_API int kvssd_b200_attention_weights_scratch_size(int queries, int n_
  * it. query [queries, query_heads, head_dim]; a place counts for query t when its row lies before
  * the block's valid count and i < visible[t] (NULL: all). lse [queries, query_heads]: given
  * (lse_given nonzero, as kvssd_b200_decode returns it), or computed and written (-inf for a query
- * that sees nothing, which then adds nothing). Blocks may be selected several times. Each output
+ * that sees nothing, which then adds nothing whatever its elements hold). Blocks may be selected several times. Each output
  * is summed in a fixed order. No reference counterpart (the reference selects blocks by their
  * order only, src/kvssd/selectors.py:11-28). */
 KVSSD_B200_API int kvssd_b200_attention_weights(const void* query, int query_dtype, int queries,
