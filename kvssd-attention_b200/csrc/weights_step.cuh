@@ -67,8 +67,9 @@ __global__ void __launch_bounds__(kThreads, step_resident(D, LO)) weights_step_k
   // one scale per unit, or `groups` of them a row
   const int groups = GROUPED ? D / a.group : S::kUnits;
   const int run = blockIdx.x * j.tiles_per_cta;
-  const int tiles = sub < subs ? min(j.total_tiles - run, j.tiles_per_cta) : 0;
-  const int count = tiles > sub ? (tiles - sub + subs - 1) / subs : 0;  // of this warp
+  const int tiles = min(j.total_tiles - run, j.tiles_per_cta);  // of the CTA: every thread looks some up
+  // of this warp; none for a warp left over where the heads do not divide the warps
+  const int count = sub < subs && tiles > sub ? (tiles - sub + subs - 1) / subs : 0;
   Tile* tile_of = reinterpret_cast<Tile*>(smem);
   uint8_t* ring = smem + j.tiles_per_cta * sizeof(Tile) + warp * kStepStages * kStage;
   const uint32_t ring_at = smem_addr(ring);
