@@ -92,8 +92,8 @@ __global__ void __launch_bounds__(kThreads) weights_lse_kernel(const WeightsArgs
       float k[kMaxPerLane];
       for (int i = 0; i < kMaxPerLane; ++i) k[i] = keys[p][lane + 32 * i];
       const float s = score(a, t, head, lane, k);
-      const float top = max(m, s);
-      if (top == -INFINITY) continue;
+      if (s == -INFINITY) continue;
+      const float top = max(m, s);  // of the numbers: a NaN score reaches l, and stays in it
       l = l * expf(m - top) + expf(s - top);
       m = top;
     }
@@ -106,6 +106,14 @@ __global__ void __launch_bounds__(kThreads) weights_lse_kernel(const WeightsArgs
   }
 }
 
+// (m, l) joined with another such part. One that has seen nothing has l = 0; a NaN in l stays.
+__device__ __forceinline__ void join(float& m, float& l, float m2, float l2) {
+  if (l2 == 0.f) return;
+  const float top = max(m, m2);
+  l = (l == 0.f ? 0.f : l * expf(m - top)) + l2 * expf(m2 - top);
+  m = top;
+}
+
 // One warp a query row: lse = log sum_parts l e^m (-inf where the row sees nothing).
 __global__ void __launch_bounds__(kThreads) weights_combine_kernel(const WeightsArgs a, int parts) {
   const int lane = threadIdx.x & 31;
@@ -116,19 +124,14 @@ __global__ void __launch_bounds__(kThreads) weights_combine_kernel(const Weights
   float m = -INFINITY, l = 0.f;
   for (int p = lane; p < parts; p += 32) {
     const float* part = a.scratch + 2 * (static_cast<long long>(p) * rows + row);
-    const float top = max(m, part[0]);
-    if (top == -INFINITY) continue;
-    l = l * expf(m - top) + part[1] * expf(part[0] - top);
-    m = top;
+    join(m, l, part[0], part[1]);
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
     const float m2 = __shfl_xor_sync(0xffffffffu, m, o), l2 = __shfl_xor_sync(0xffffffffu, l, o);
-    const float top = max(m, m2);
-    if (top != -INFINITY) l = l * expf(m - top) + l2 * expf(m2 - top);
-    m = top;
+    join(m, l, m2, l2);
   }
-  if (lane == 0) a.lse[row] = m == -INFINITY ? -INFINITY : m + logf(l);
+  if (lane == 0) a.lse[row] = l == 0.f ? -INFINITY : m + logf(l);
 }
 
 __global__ void __launch_bounds__(kThreads) weights_kernel(const WeightsArgs a) {

@@ -79,7 +79,7 @@ def attention_weights(query, packed_k, scales_k, valid, bits, group, sm_scale, l
     else:
         full = np.asarray(lse, np.float64).reshape(t, kvh, -1).transpose(1, 0, 2)
     with np.errstate(invalid="ignore"):
-        p = np.where((full == -np.inf)[..., None], 0.0, np.exp(score - full[..., None]))
+        p = np.where((full == -np.inf)[..., None] | ~seen[None, :, None], 0.0, np.exp(score - full[..., None]))
     w = p.sum((1, 2))
     if previous is not None:
         w = w + previous

@@ -12,6 +12,7 @@ import torch
 
 from kvssd_b200 import ops
 from kvssd_b200.quant import quantize_tensor
+from oracle import cache_oracle as orc
 
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda", 0)
@@ -50,3 +51,54 @@ def test_weights_step_many_short_blocks_of_uneven_heads(kvh, places, d, bits, gr
     many, _ = ops.attention_weights(query, kp, ks, valid, bits, group, scale, lse=lse, block_table=table)
     assert torch.equal(many, once[:, table.long()])
     assert ops.read_device_status(DEV) == 0
+
+
+def check_nan(query, kp, ks, valid, bits, group, scale, visible=None):
+    """NaN exactly where the 64-bit form has it; elsewhere scores of order one, whose FP32 sums of up to
+    256 products are off by less than 2^-13: 1e-3 of a weight, absolutely of a log-sum-exp."""
+    out, lse = ops.attention_weights(query, kp, ks, valid, bits, group, scale, visible=visible)
+    cpu = lambda t: None if t is None else t.cpu().numpy()  # noqa: E731
+    w, full, _ = orc.attention_weights(query.double().cpu().numpy(), cpu(kp), cpu(ks), cpu(valid), bits, group,
+                                       scale, visible=cpu(visible))
+    for got, want in ((out.double().cpu().numpy(), w), (lse.double().cpu().numpy(), full)):
+        assert (np.isnan(got) == np.isnan(want)).all()
+        np.testing.assert_allclose(got, want, rtol=1e-3, atol=1e-3 if want is full else 1e-30)
+    return out, lse
+
+
+NAN_SHAPES = [  # gqa, d, bits, group, queries: forms for any shape, for steps, windows and long windows
+    (2, 32, 4, 8, 2), (1, 80, 2, 40, 3), (12, 36, 4, 12, 5), (2, 128, 4, 32, 2), (3, 64, 2, 16, 2),
+    (4, 128, 2, 32, 5), (4, 96, 4, 48, 6), (10, 128, 4, 32, 5), (10, 64, 2, 32, 4), (40, 256, 2, 64, 2)]
+
+
+@pytest.mark.filterwarnings("ignore::RuntimeWarning")
+@pytest.mark.parametrize("shape", NAN_SHAPES)
+def test_weights_nan_scores_show(shape):
+    """A NaN in a query or in a key's scale shows in all that sees it, whichever place it has among the
+    keys, and in nothing else."""
+    gqa, d, bits, group, queries = shape
+    kvh, nb, bt = 2, 5, 40
+    n = nb * bt
+    kp, ks = key_pool(nb, bt, kvh, d, bits, group, 3)
+    valid = torch.full((nb,), bt, dtype=torch.int32, device=DEV)
+    clean = torch.randn(queries, kvh * gqa, d, generator=gen(4)).to(DEV)
+    scale = 1 / math.sqrt(d)
+    query = clean.clone()
+    query[-1, gqa, 1] = math.nan  # the last query's first head of KV head 1
+    _, lse = check_nan(query, kp, ks, valid, bits, group, scale)
+    assert lse.isnan().sum() == 1
+    seen = torch.full((queries,), n, dtype=torch.int32, device=DEV)
+    seen[-1] = 70
+    out, _ = check_nan(query, kp, ks, valid, bits, group, scale, visible=seen)
+    assert out[1, :70].isnan().all() and not out[1, 70:].isnan().any() and not out[0].isnan().any()
+    for place in (0, 32, 45, 63, n - 1):  # first, later and last places of a run of 32, of all
+        broken = ks.clone()
+        broken[place // bt, place % bt, 0, -1] = math.nan
+        out, lse = check_nan(clean, kp, broken, valid, bits, group, scale)
+        assert out[0].isnan().all() and not out[1].isnan().any()
+        seen = torch.full((queries,), n, dtype=torch.int32, device=DEV)
+        seen[0] = place  # the first query sees the places before it only
+        check_nan(clean, kp, broken, valid, bits, group, scale, visible=seen)
+    valid[-1] = bt - 1  # behind the valid rows it does not show
+    out, lse = check_nan(clean, kp, broken, valid, bits, group, scale)
+    assert not out.isnan().any() and not lse.isnan().any()
