@@ -506,6 +506,8 @@ class _StatusWatch:
         self._next += 1
 
     def poll(self, where: str) -> None:
+        if torch.cuda.is_current_stream_capturing():
+            return  # an event must not be queried then; a later call outside looks
         value = 0
         for i in range(self.SLOTS):
             value |= self._take(i, block=False)

@@ -10,7 +10,7 @@ import numpy as np
 import pytest
 import torch
 
-from kvssd_b200 import ops
+from kvssd_b200 import CacheSpec, DeviceBlockPool, DeviceKVCache, ops
 from kvssd_b200.quant import quantize_tensor
 from oracle import cache_oracle as orc
 
@@ -102,3 +102,39 @@ def test_weights_nan_scores_show(shape):
     valid[-1] = bt - 1  # behind the valid rows it does not show
     out, lse = check_nan(clean, kp, broken, valid, bits, group, scale)
     assert not out.isnan().any() and not lse.isnan().any()
+
+
+# ------------------------------------------------------------------------------------ DeviceKVCache
+
+
+SPEC = CacheSpec(layers=1, kv_heads=2, head_dim=64, block_tokens=8, bits=4, group_size=32)
+
+
+def small_cache(tokens=13, blocks=4, rotary=None):
+    cache = DeviceKVCache(SPEC, blocks, DEV, rotary)
+    x = torch.randn(tokens, 2, 64, generator=gen(tokens)).half().to(DEV)
+    cache.append(x, x)
+    return cache
+
+
+@pytest.mark.parametrize("pooled", [False, True])
+def test_decode_captured_behind_decodes_on_the_same_stream(pooled):
+    """The reads of the status word that earlier decodes left outstanding do not disturb a capture."""
+    holder = small_cache()
+    if pooled:
+        holder = DeviceBlockPool(SPEC, *(t[:2] for t in (holder.packed_k, holder.packed_v, holder.scales_k,
+                                                         holder.scales_v, holder.valid_tokens)))
+    query = torch.randn(4, 64, generator=gen(2)).half().to(DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            ref = holder.decode(query)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        out = holder.decode(query)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out[0], ref[0]) and torch.equal(out[1], ref[1])
+    with torch.cuda.stream(side):
+        holder.check()
