@@ -143,7 +143,8 @@ class DeviceKVCache:
     def observe(self, query: torch.Tensor, sm_scale: float | None = None) -> torch.Tensor:
         """Adds the weights that the last T tokens' queries [T, query_heads, head_dim] (not yet
         rotated) give the cache, each seeing the places up to its own token; returns their
-        log-sum-exps [T, query_heads]. For a prompt, before anything has been evicted."""
+        log-sum-exps [T, query_heads]. For a prompt, before anything has been evicted. Asynchronous, as
+        ``decode`` is; after a failure ``weights`` hold NaN."""
         if query.ndim != 3 or not 1 <= query.shape[0] <= self.n_tokens:
             raise ValueError("query must be [T, query_heads, head_dim] of the last T tokens")
         if self.next_position != self.n_tokens:
@@ -152,16 +153,20 @@ class DeviceKVCache:
         t, n = query.shape[0], self.n_tokens
         visible = torch.arange(n - t + 1, n + 1, dtype=torch.int32, device=self.device)
         weights = self.weights[:, :b * self.spec.block_tokens]
+        watch = ops.status_watch(self.device)
+        watch.poll("DeviceKVCache.observe (an earlier call)")
         _, lse = ops.attention_weights(self._rotated(query), packed_k, scales_k, valid,
                                        self.spec.bits, self.spec.group_size, self._scale(sm_scale),
                                        visible=visible, previous=weights, out=weights)
+        watch.arm("DeviceKVCache.observe")
         return lse
 
     def evict(self, keep: int, sink: int = 0, recent: int = 0, shared: bool = False) -> None:
         """Keeps ``keep`` tokens per KV head (or the same for all, ``shared``): the first ``sink``
         positions, the ``recent`` latest, and those of the largest accumulated weight (ops.evict).
         A cache that holds no more than ``keep`` tokens is left as it is. Once the heads have chosen
-        for themselves, a shared choice has no meaning any more and is refused."""
+        for themselves, a shared choice has no meaning any more and is refused. A failure of an earlier
+        call that is known by now is raised before anything moves; ``check()`` first waits for all."""
         if keep < 1 or sink < 0 or recent < 0:
             raise ValueError("keep must be positive, sink and recent non-negative")
         if shared and self._own_choices:
@@ -169,6 +174,7 @@ class DeviceKVCache:
         if self.n_tokens <= keep:
             return
         b = self.used_blocks
+        ops.status_watch(self.device).poll("DeviceKVCache.evict (an earlier call)")
         self.weights, self.positions = ops.evict(
             self.weights, self.positions, self.n_tokens, keep, self.packed_k[:b], self.packed_v[:b],
             self.scales_k[:b], self.scales_v[:b], self.valid_tokens[:b], sink=sink, recent=recent,
@@ -177,6 +183,8 @@ class DeviceKVCache:
         self._own_choices |= not shared
 
     def check(self) -> None:
-        """Waits for the outstanding status reads of this device's current stream and raises
-        ops.DeviceFailure if a call flagged a failure."""
-        ops.status_watch(self.device).check("DeviceKVCache")
+        """Waits for this device's current stream and raises ops.DeviceFailure if any call on it flagged
+        a failure."""
+        watch = ops.status_watch(self.device)
+        watch.arm("DeviceKVCache")  # behind all calls, those that arm no read of their own included
+        watch.check("DeviceKVCache")

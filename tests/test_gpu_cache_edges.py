@@ -10,7 +10,7 @@ import numpy as np
 import pytest
 import torch
 
-from kvssd_b200 import CacheSpec, DeviceBlockPool, DeviceKVCache, ops
+from kvssd_b200 import CacheSpec, DeviceBlockPool, DeviceKVCache, _native, ops
 from kvssd_b200.quant import quantize_tensor
 from oracle import cache_oracle as orc
 
@@ -138,3 +138,43 @@ def test_decode_captured_behind_decodes_on_the_same_stream(pooled):
     assert torch.equal(out[0], ref[0]) and torch.equal(out[1], ref[1])
     with torch.cuda.stream(side):
         holder.check()
+
+
+def status_word():
+    """The status word of the current stream's workspace, as the kernels see it."""
+    return ops._workspaces.get(DEV, torch.cuda.current_stream(DEV), 2048)[:4].view(torch.int32)
+
+
+def test_cache_check_reports_a_failed_window():
+    """A window whose wait gave up has set its bit and left NaN; check() raises, and clears it."""
+    ops.read_device_status(DEV)
+    cache = small_cache()
+    query = torch.randn(3, 4, 64, generator=gen(1)).half().to(DEV)
+    status_word().fill_(_native.DEV_STREAM_TIMEOUT)
+    cache.observe(query)
+    with pytest.raises(ops.DeviceFailure, match="gave up"):
+        cache.check()
+    cache.check()
+    # flagged by a call that arms no read of its own
+    status_word().fill_(_native.DEV_BAD_BLOCK)
+    with pytest.raises(ops.DeviceFailure, match="outside the pool"):
+        cache.check()
+    assert ops.read_device_status(DEV) == 0
+
+
+@pytest.mark.parametrize("call", ["observe", "evict"])
+def test_cache_raises_a_known_failure_before_the_next_call(call):
+    ops.read_device_status(DEV)
+    cache = small_cache()
+    query = torch.randn(3, 4, 64, generator=gen(1)).half().to(DEV)
+    status_word().fill_(_native.DEV_STREAM_TIMEOUT)
+    cache.observe(query)
+    torch.cuda.synchronize()
+    before = [t.clone() for t in (cache.packed_k, cache.weights, cache.positions)]
+    with pytest.raises(ops.DeviceFailure, match=call):
+        cache.evict(5) if call == "evict" else cache.observe(query)
+    assert cache.n_tokens == 13
+    assert all(torch.equal(a, b) for a, b in zip(before, (cache.packed_k, cache.weights, cache.positions)))
+    cache.evict(5)
+    cache.check()
+    assert cache.n_tokens == 5
