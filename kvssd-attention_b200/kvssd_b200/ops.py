@@ -31,11 +31,14 @@ class _Workspaces:
     Reuse is safe because calls that share a workspace are ordered on one stream. A workspace
     is zeroed once at allocation: the header's device status word (it accumulates until read),
     the fused combine's epoch and the part words, whose epoch tags must not match a future call.
+    A workspace that a larger one replaces is kept: a captured graph may hold its address, for its
+    parts or for its status word. As sizes double, all of them are smaller than the one in use.
     """
 
     def __init__(self) -> None:
         self._lock = threading.Lock()
         self._buffers: dict[tuple[int, int], torch.Tensor] = {}
+        self._replaced: dict[tuple[int, int], list[torch.Tensor]] = {}
 
     def get(self, device: torch.device, stream: torch.cuda.Stream, nbytes: int) -> torch.Tensor:
         key = (device.index, stream.cuda_stream)
@@ -45,9 +48,22 @@ class _Workspaces:
                 size = max(nbytes, 1 << 20)
                 if buf is not None:
                     size = max(size, 2 * buf.numel())
-                buf = torch.zeros(size, dtype=torch.uint8, device=device)
+                old, buf = buf, torch.zeros(size, dtype=torch.uint8, device=device)
+                if old is not None:
+                    self._replaced.setdefault(key, []).append(old)
+                    if not torch.cuda.is_current_stream_capturing():
+                        buf[:4].copy_(old[:4])  # what has been flagged and not been read
                 self._buffers[key] = buf
             return buf
+
+    def status_words(self, device_index: int, stream: int | None = None) -> list[torch.Tensor]:
+        """The workspaces of one stream (None: of every stream) of a device, replaced ones included:
+        a replayed graph flags what it finds in the one it was captured with."""
+        with self._lock:
+            return [buf for key, buf in self._buffers.items()
+                    if key[0] == device_index and stream in (None, key[1])] + [
+                buf for key, bufs in self._replaced.items()
+                if key[0] == device_index and stream in (None, key[1]) for buf in bufs]
 
 
 _workspaces = _Workspaces()
@@ -389,28 +405,15 @@ def read_device_status(device: torch.device | str | None = None, clear: bool = T
     """
     device = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
     stream = stream or torch.cuda.current_stream(device)
-    ws = _workspaces.get(device, stream, _WORKSPACE_HEADER)
-    value = ctypes.c_uint()
-    with torch.cuda.device(device):
-        status = _native.library().kvssd_b200_read_status(
-            _ptr(ws), 1 if clear else 0, ctypes.byref(value), stream.cuda_stream
-        )
-    if status not in (_native.OK, _native.ERR_DEVICE_STATUS):
-        _native.check(status, "kvssd_b200_read_status")
-    return int(value.value)
+    _workspaces.get(device, stream, _WORKSPACE_HEADER)
+    return _read_words(device, _workspaces.status_words(device.index, stream.cuda_stream), clear, stream)
 
 
-def read_device_status_all(device: torch.device | str | None = None, clear: bool = True) -> int:
-    """OR of the status words of every decode workspace on ``device`` (one per stream that has
-    decoded, graph-capture streams included), read after synchronising the device."""
-    device = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
-    torch.cuda.synchronize(device)
-    with _workspaces._lock:
-        buffers = [buf for (dev, _), buf in _workspaces._buffers.items() if dev == device.index]
+def _read_words(device: torch.device, workspaces: list[torch.Tensor], clear: bool,
+                stream: torch.cuda.Stream) -> int:
     total = 0
-    stream = torch.cuda.current_stream(device)
     with torch.cuda.device(device):
-        for ws in buffers:
+        for ws in workspaces:
             value = ctypes.c_uint()
             status = _native.library().kvssd_b200_read_status(
                 _ptr(ws), 1 if clear else 0, ctypes.byref(value), stream.cuda_stream)
@@ -418,6 +421,15 @@ def read_device_status_all(device: torch.device | str | None = None, clear: bool
                 _native.check(status, "kvssd_b200_read_status")
             total |= int(value.value)
     return total
+
+
+def read_device_status_all(device: torch.device | str | None = None, clear: bool = True) -> int:
+    """OR of the status words of every decode workspace on ``device`` (one per stream that has
+    decoded, graph-capture streams included), read after synchronising the device."""
+    device = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
+    torch.cuda.synchronize(device)
+    return _read_words(device, _workspaces.status_words(device.index), clear,
+                       torch.cuda.current_stream(device))
 
 
 # Status bits that make a call's result invalid (the kernels then write NaN into out/lse) or

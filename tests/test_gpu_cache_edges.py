@@ -178,3 +178,31 @@ def test_cache_raises_a_known_failure_before_the_next_call(call):
     cache.evict(5)
     cache.check()
     assert cache.n_tokens == 5
+
+
+def test_a_graph_flags_in_a_workspace_that_has_been_replaced():
+    """A captured call's status word outlives the workspace that held it; its flag is still read."""
+    pool = [torch.zeros(2, 4, 1, 16, dtype=torch.uint8, device=DEV) for _ in "kv"] + [
+        torch.zeros(2, 4, 1, 1, dtype=torch.float16, device=DEV) for _ in "kv"]
+    x = torch.randn(2, 1, 32, generator=gen(1)).to(DEV)
+    slots = torch.tensor([1, 3], device=DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ops.append(x, x, slots, *pool, 4, 32)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        ops.append(x, x, slots, *pool, 4, 32)
+    with torch.cuda.stream(side):
+        held = ops._workspaces.get(DEV, side, 2048)
+        ops._workspaces.get(DEV, side, 4 * held.numel())
+    del held
+    torch.cuda.synchronize()
+    slots[1] = 8  # behind the pool
+    graph.replay()
+    torch.cuda.synchronize()
+    assert ops.read_device_status(DEV, stream=side) == _native.DEV_BAD_BLOCK
+    assert ops.read_device_status(DEV, stream=side) == 0
+    graph.replay()
+    assert ops.read_device_status_all(DEV) & _native.DEV_BAD_BLOCK
+    assert ops.read_device_status_all(DEV) == 0
