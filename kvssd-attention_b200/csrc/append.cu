@@ -176,7 +176,8 @@ __device__ __forceinline__ float reciprocal(float x) {
 
 // a / b rounded to nearest, given b's reciprocal: two steps of Markstein's (1990) from a * inverse, each
 // adding the remainder (exact in an FMA) times the inverse; the first brings the quotient within an
-// ulp, the second rounds it. Quotients here are 0 or far from FP32's limits.
+// ulp, the second rounds it. The inverse must not be subnormal: b is below 2^126. Quotients here are 0 or
+// far from FP32's limits.
 __device__ __forceinline__ F2 quotient(F2 a, F2 b, F2 inverse) {
   const F2 minus = mul2(b, f2(-1.f));
   F2 q = mul2(a, inverse);
@@ -185,14 +186,18 @@ __device__ __forceinline__ F2 quotient(F2 a, F2 b, F2 inverse) {
 }
 
 // Quantizes 8 elements of one group: codes 0 .. 2^bits - 1 as floats. Adding 1.5 2^23 + mid rounds the
-// quotient half to even and adds the (even) midpoint.
+// quotient half to even and adds the (even) midpoint. An INT4 scale is below 2^128 / 7; an INT2 one may be
+// any finite number, so its quotients are taken by a quarter of it, and divided by 4 as they are rounded.
 template <int BITS>
 __device__ __forceinline__ void quantize8(const F2 (&x)[4], float scale, F2 (&code)[4]) {
-  constexpr float kRound = 12582912.f;
-  const F2 b = f2(scale), inverse = f2(reciprocal(scale));
+  constexpr float kPart = BITS == 2 ? 0.25f : 1.f;
+  const F2 round = f2(12582912.f + (1 << (BITS - 1)));
+  const F2 b = f2(scale * kPart), inverse = f2(reciprocal(scale * kPart));
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    code[i] = add2(add2(quotient(x[i], b, inverse), f2(kRound + (1 << (BITS - 1)))), f2(-kRound));
+  for (int i = 0; i < 4; ++i) {
+    const F2 q = quotient(x[i], b, inverse);
+    code[i] = add2(BITS == 2 ? fma2(q, f2(kPart), round) : add2(q, round), f2(-12582912.f));
+  }
 }
 
 // max|x| / (2^(bits-1) - 1), at least 1e-8 over that.

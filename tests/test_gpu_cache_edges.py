@@ -104,6 +104,42 @@ def test_weights_nan_scores_show(shape):
     assert not out.isnan().any() and not lse.isnan().any()
 
 
+# ------------------------------------------------------------------------------------------ append
+
+
+def make_pool(nb, bt, kvh, d, bits, group):
+    return [torch.zeros(nb, bt, kvh, d * bits // 8, dtype=torch.uint8, device=DEV) for _ in "kv"] + [
+        torch.zeros(nb, bt, kvh, d // group, dtype=torch.float16, device=DEV) for _ in "kv"]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("bits", [2, 4])
+@pytest.mark.parametrize("d, group, kvh", [(128, 32, 2), (64, 64, 3), (128, 16, 1), (20, 4, 2)])
+def test_append_at_the_end_of_fp32(d, group, kvh, bits, dtype):
+    """Groups whose largest element lies between 2^120 and the largest number of the type, and groups of the
+    smallest: codes and scales (infinite in FP16 at the top) are the quantizer's."""
+    top = torch.finfo(dtype).max
+    tokens = 40
+    x = torch.rand(tokens, kvh, d, generator=gen(bits)) * 2 - 1
+    size = 2.0 ** torch.linspace(-149, 127.9, tokens - 4)
+    x[4:] *= size[:, None, None]
+    x[0] *= top
+    x[1] *= top / 2
+    x[1, :, 0::group] = top
+    x[2] *= 2.0**125
+    x[2, :, 1::group] = -(2.0**126)
+    x[3] *= 2.0**126
+    x[3, :, 1::group] = 2.0**126 * 1.0078125
+    x = x.to(dtype)
+    assert x.isfinite().all()
+    pool = make_pool(5, 8, kvh, d, bits, group)
+    ops.append(x.to(DEV), (-x).to(DEV), torch.arange(tokens, device=DEV), *pool, bits, group)
+    for i, y in enumerate((x, -x)):
+        q = quantize_tensor(y.float(), bits, group)
+        assert torch.equal(pool[i].flatten(0, 1).cpu(), q.packed)
+        assert torch.equal(pool[2 + i].flatten(0, 1).cpu(), q.scales)
+
+
 # ------------------------------------------------------------------------------------ DeviceKVCache
 
 
