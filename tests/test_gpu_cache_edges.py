@@ -140,6 +140,29 @@ def test_append_at_the_end_of_fp32(d, group, kvh, bits, dtype):
         assert torch.equal(pool[2 + i].flatten(0, 1).cpu(), q.scales)
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("tokens, kvh, d, bits, group, pairs", [
+    (37, 2, 128, 4, 32, 64), (300, 8, 128, 2, 32, 32), (9, 3, 20, 4, 4, 7), (1200, 1, 64, 4, 16, 32)])
+def test_append_with_a_magnitude(tokens, kvh, d, bits, group, pairs, dtype, interleaved):
+    """Keys rotated with cos and sin times a magnitude (taken in FP32, as the entry point does)."""
+    magnitude = float(np.float32(0.1 * math.log(4.0) + 1.0))
+    g = gen(tokens + d)
+    key, value = [(torch.randn(tokens, kvh, d, generator=g) * 2).to(dtype) for _ in "kv"]
+    positions = torch.arange(tokens) * 7 + 54_321
+    f = 10000.0 ** (-torch.arange(pairs, dtype=torch.float64) / pairs)
+    nb = -(-tokens // 16)
+    pool = make_pool(nb, 16, kvh, d, bits, group)
+    ops.append(key.to(DEV), value.to(DEV), torch.arange(tokens, device=DEV), *pool, bits, group,
+               positions=positions.to(DEV), frequencies=f.to(DEV), interleaved=interleaved,
+               magnitude=magnitude)
+    turned = orc.rotate(key.double().numpy(), positions.numpy(), f.numpy(), interleaved, magnitude)
+    for i, y in enumerate((torch.from_numpy(turned.astype(np.float32)), value.float())):
+        q = quantize_tensor(y, bits, group)
+        assert torch.equal(pool[i].flatten(0, 1)[:tokens].cpu(), q.packed)
+        assert torch.equal(pool[2 + i].flatten(0, 1)[:tokens].cpu(), q.scales)
+
+
 # ------------------------------------------------------------------------------------ DeviceKVCache
 
 
