@@ -113,7 +113,7 @@ int kvssd_b200_attention_weights_scratch_size(int queries, int n_sel_blocks, int
   if (int st = check_cache(1, block_tokens, kv_heads, head_dim, bits, group_size)) return st;
   if (int st = check_places(n_sel_blocks, block_tokens)) return st;
   if (queries < 1 || query_heads < 1) return bad("all dimensions must be positive");
-  *bytes = weights_scratch_bytes(queries, query_heads, n_sel_blocks, block_tokens);
+  *bytes = weights_scratch_bytes(queries, query_heads, kv_heads, n_sel_blocks, block_tokens, head_dim, group_size);
   return KVSSD_B200_OK;
 }
 
@@ -138,13 +138,16 @@ int kvssd_b200_attention_weights(const void* query, int query_dtype, int queries
     return bad("tensor pointers must not be NULL");
   if (static_cast<long long>(queries) * query_heads > 0x1000000ll)
     return report(KVSSD_B200_ERR_UNSUPPORTED, "more than 2^24 query rows are not supported");
-  if (!lse_given && (!scratch || scratch_bytes < weights_scratch_bytes(queries, query_heads, n_sel_blocks, block_tokens)))
+  if (!lse_given && (!scratch || scratch_bytes < weights_scratch_bytes(queries, query_heads, kv_heads, n_sel_blocks,
+                                                                       block_tokens, head_dim, group_size)))
     return report(KVSSD_B200_ERR_WORKSPACE, "scratch missing or too small");
   WeightsArgs a{query, query_dtype, queries, query_heads, packed_k,
                 reinterpret_cast<const __half*>(scales_k), valid_tokens, block_table, visible,
                 n_pool_blocks, n_sel_blocks, block_tokens, kv_heads, head_dim, bits, group_size,
                 sm_scale, lse_given ? lse : nullptr, lse, previous, previous_stride, out, out_stride,
-                static_cast<float*>(scratch), device_status};
+                static_cast<float*>(scratch),
+                static_cast<long long>(scratch_bytes / (2 * sizeof(float))) / (static_cast<long long>(queries) * query_heads),
+                device_status};
   return launched(launch_weights(a, reinterpret_cast<cudaStream_t>(stream)),
                   "attention weights launch failed");
 }

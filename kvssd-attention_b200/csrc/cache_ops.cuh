@@ -74,6 +74,7 @@ struct WeightsArgs {
   float* out;
   long long out_stride;
   float* scratch;          // parts of the log-sum-exps when computed
+  long long parts_room;    // as many a query row as it holds
   unsigned* status;
 };
 
@@ -106,7 +107,7 @@ int report(int status, const char* message);
 
 cudaError_t launch_rotary(const RotaryArgs& a, cudaStream_t s);
 cudaError_t launch_append(const AppendArgs& a, cudaStream_t s);
-size_t weights_scratch_bytes(int queries, int qh, int n_sel, int bt);
+size_t weights_scratch_bytes(int queries, int qh, int kvh, int n_sel, int bt, int d, int group);
 cudaError_t launch_weights(const WeightsArgs& a, cudaStream_t s);
 size_t evict_scratch_ints(int n, int lists);
 cudaError_t launch_evict(const EvictArgs& a, cudaStream_t s);

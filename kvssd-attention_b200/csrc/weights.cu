@@ -10,7 +10,7 @@
 // weights_umma.cuh. weights_lse_kernel, weights_combine_kernel and weights_kernel are the
 // form for any other shape: a CTA takes one KV head and kPlaces places, a warp one place at a time,
 // the lanes the head's dims.
-#include "weights_tc.cuh"
+#include "weights_umma.cuh"
 
 namespace kvb {
 namespace {
@@ -67,51 +67,58 @@ __device__ __forceinline__ bool sees(const WeightsArgs& a, int t, int place) {
   return !a.visible || place < a.visible[t];
 }
 
-// Parts (m, l) of each query row over one run of kPlaces places: scratch [chunks][rows][2].
-__global__ void __launch_bounds__(kThreads) weights_lse_kernel(const WeightsArgs a) {
-  __shared__ float keys[kPlaces][kMaxPerLane * 32];
-  __shared__ bool live[kPlaces];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int h = blockIdx.y, first = blockIdx.x * kPlaces, gqa = a.qh / a.kvh;
-  const int places = min(kPlaces, a.n_sel * a.bt - first);
-  pdl_wait();
-  pdl_launch();
-  for (int p = warp; p < places; p += kWarps) {
-    float k[kMaxPerLane];
-    const bool ok = load_key(a, first + p, h, lane, k);
-    if (lane == 0) live[p] = ok;
-    if (ok)
-      for (int i = 0; i < kMaxPerLane; ++i) keys[p][lane + 32 * i] = k[i];
-  }
-  __syncthreads();
-  for (int r = warp; r < a.queries * gqa; r += kWarps) {
-    const int t = r / gqa, head = h * gqa + r % gqa;
-    float m = -INFINITY, l = 0.f;
-    for (int p = 0; p < places; ++p) {
-      if (!live[p] || !sees(a, t, first + p)) continue;
-      float k[kMaxPerLane];
-      for (int i = 0; i < kMaxPerLane; ++i) k[i] = keys[p][lane + 32 * i];
-      const float s = score(a, t, head, lane, k);
-      if (s == -INFINITY) continue;
-      const float top = max(m, s);  // of the numbers: a NaN score reaches l, and stays in it
-      l = l * expf(m - top) + expf(s - top);
-      m = top;
-    }
-    if (lane == 0) {
-      float* part = a.scratch + 2 * (static_cast<long long>(blockIdx.x) * a.queries * a.qh +
-                                     static_cast<long long>(t) * a.qh + head);
-      part[0] = m;
-      part[1] = l;
-    }
-  }
-}
-
 // (m, l) joined with another such part. One that has seen nothing has l = 0; a NaN in l stays.
 __device__ __forceinline__ void join(float& m, float& l, float m2, float l2) {
   if (l2 == 0.f) return;
   const float top = max(m, m2);
   l = (l == 0.f ? 0.f : l * expf(m - top)) + l2 * expf(m2 - top);
   m = top;
+}
+
+// Parts (m, l) of each query row: scratch [parts][rows][2]. A CTA takes the run of kPlaces places of its
+// number or, RUNS, every gridDim.x-th one from it on, and joins what it finds with what it has found before.
+template <bool RUNS>
+__global__ void __launch_bounds__(kThreads) weights_lse_kernel(const WeightsArgs a, int chunks) {
+  __shared__ float keys[kPlaces][kMaxPerLane * 32];
+  __shared__ bool live[kPlaces];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int h = blockIdx.y, gqa = a.qh / a.kvh;
+  pdl_wait();
+  pdl_launch();
+  for (int chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
+    const int first = chunk * kPlaces, places = min(kPlaces, a.n_sel * a.bt - first);
+    for (int p = warp; p < places; p += kWarps) {
+      float k[kMaxPerLane];
+      const bool ok = load_key(a, first + p, h, lane, k);
+      if (lane == 0) live[p] = ok;
+      if (ok)
+        for (int i = 0; i < kMaxPerLane; ++i) keys[p][lane + 32 * i] = k[i];
+    }
+    __syncthreads();
+    for (int r = warp; r < a.queries * gqa; r += kWarps) {
+      const int t = r / gqa, head = h * gqa + r % gqa;
+      float m = -INFINITY, l = 0.f;
+      for (int p = 0; p < places; ++p) {
+        if (!live[p] || !sees(a, t, first + p)) continue;
+        float k[kMaxPerLane];
+        for (int i = 0; i < kMaxPerLane; ++i) k[i] = keys[p][lane + 32 * i];
+        const float s = score(a, t, head, lane, k);
+        if (s == -INFINITY) continue;
+        const float top = max(m, s);  // of the numbers: a NaN score reaches l, and stays in it
+        l = l * expf(m - top) + expf(s - top);
+        m = top;
+      }
+      if (lane == 0) {
+        float* part = a.scratch + 2 * (static_cast<long long>(blockIdx.x) * a.queries * a.qh +
+                                       static_cast<long long>(t) * a.qh + head);
+        if (RUNS && chunk >= gridDim.x) join(m, l, part[0], part[1]);
+        part[0] = m;
+        part[1] = l;
+      }
+    }
+    if (!RUNS) break;
+    __syncthreads();
+  }
 }
 
 // One warp a query row: lse = log sum_parts l e^m (-inf where the row sees nothing).
@@ -175,11 +182,28 @@ TcLauncher tc_launcher(int d, int group) {
   }
 }
 
-size_t weights_scratch_bytes(int queries, int qh, int n_sel, int bt) {
-  // the general form's parts; those of the tensor-core form, at most one per 32 places too
+// Parts of a query row in the log-sum-exp pass for any shape: one a run of places (131072 places x 8 heads of
+// 80: 1.68 ms; as many as are resident at once, each of several runs, 1.83 ms) up to 8 MB of them in all, or
+// as many as are resident.
+long long general_parts(int queries, int qh, int kvh, int n_sel, int bt) {
   const long long chunks = (static_cast<long long>(n_sel) * bt + kPlaces - 1) / kPlaces;
-  const long long tiles = static_cast<long long>(n_sel) * ((bt + 31) / 32);
-  const long long parts = chunks > tiles ? chunks : tiles;
+  long long most = (1ll << 20) / (static_cast<long long>(queries) * qh);
+  if (most < 148 * 4 / kvh) most = 148 * 4 / kvh;
+  if (most < 1) most = 1;
+  return most < chunks ? most : chunks;
+}
+
+size_t weights_scratch_bytes(int queries, int qh, int kvh, int n_sel, int bt, int d, int group) {
+  long long parts = general_parts(queries, qh, kvh, n_sel, bt);  // of any shape off 16 bytes too
+  if (tc_launcher(d, group)) {
+    const int tiles = n_sel * ((bt + 15) / 16);  // of the narrower windows, at most
+    const int window = weights_tc::grid_x(tiles, kvh, 1, weights_tc::kWarps, 2);
+    parts = window > parts ? window : parts;
+    for (int ctas = 1; ctas <= 2; ++ctas) {  // an SM, by the shape and the queries' type
+      const int wide = weights_umma::plan(n_sel, bt, kvh, ctas).parts;
+      parts = wide > parts ? wide : parts;
+    }
+  }
   return static_cast<size_t>(parts) * queries * qh * 2 * sizeof(float);
 }
 
@@ -189,10 +213,13 @@ cudaError_t launch_weights(const WeightsArgs& a, cudaStream_t s) {
     return tc(a, s);
   const int chunks = (a.n_sel * a.bt + kPlaces - 1) / kPlaces;
   if (!a.lse_in) {
-    cudaError_t e = launch_pdl(weights_lse_kernel, dim3(chunks, a.kvh), kThreads, 0, s, a);
+    const int parts = static_cast<int>(general_parts(a.queries, a.qh, a.kvh, a.n_sel, a.bt));
+    if (parts > a.parts_room) return cudaErrorInvalidValue;
+    cudaError_t e = launch_pdl(parts < chunks ? weights_lse_kernel<true> : weights_lse_kernel<false>,
+                               dim3(parts, a.kvh), kThreads, 0, s, a, chunks);
     if (e != cudaSuccess) return e;
     e = launch_pdl(weights_combine_kernel, dim3((a.queries * a.qh + kWarps - 1) / kWarps), kThreads,
-                   0, s, a, chunks);
+                   0, s, a, parts);
     if (e != cudaSuccess) return e;
   }
   return launch_pdl(weights_kernel, dim3(chunks, a.kvh), kThreads, 0, s, a);

@@ -19,6 +19,7 @@ cudaError_t launch_shape(const WeightsArgs& a, cudaStream_t s) {
   j.total_tiles = a.n_sel * j.tiles_per_block;
   if (!a.lse_in) {
     j.parts = grid_x(j.total_tiles, a.kvh, 1, kWarps, resident(D, LO));
+    if (j.parts > a.parts_room) return cudaErrorInvalidValue;
     const cudaError_t e = launch_mode<BITS, D, UNIT, LO, kLse>(j, s);
     if (e != cudaSuccess) return e;
   }

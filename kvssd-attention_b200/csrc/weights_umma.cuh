@@ -613,19 +613,32 @@ cudaError_t launch_pass(Job j, cudaStream_t s) {
   return cudaSuccess;
 }
 
+struct Plan {
+  int total_tiles, tiles_per_cta, parts;
+};
+inline Plan plan(int n_sel, int bt, int kvh, int ctas) {  // ctas: on an SM
+  Plan p;
+  p.total_tiles = static_cast<int>((static_cast<long long>(n_sel) * bt + kTile - 1) / kTile);
+  const int want = 148 * ctas / kvh < 1 ? 1 : 148 * ctas / kvh;
+  p.tiles_per_cta = (p.total_tiles + want - 1) / want;
+  // a run touches at most this many blocks (a partial one at either end): more CTAs otherwise
+  const long long most = static_cast<long long>(kMostSlots - 2) * bt / kTile;
+  if (p.tiles_per_cta > most) p.tiles_per_cta = most < 1 ? 1 : static_cast<int>(most);
+  p.parts = (p.total_tiles + p.tiles_per_cta - 1) / p.tiles_per_cta;
+  return p;
+}
+
 template <int BITS, int D, bool LO>
 cudaError_t launch(const WeightsArgs& a, cudaStream_t s) {
   Job j{};
   j.a = a;
   j.rows = a.queries * (a.qh / a.kvh);
-  j.total_tiles = static_cast<int>((static_cast<long long>(a.n_sel) * a.bt + kTile - 1) / kTile);
-  const int want = 148 * resident(D) / a.kvh < 1 ? 1 : 148 * resident(D) / a.kvh;
-  j.tiles_per_cta = (j.total_tiles + want - 1) / want;
-  // a run touches at most this many blocks (a partial one at either end): more CTAs otherwise
-  const long long most = static_cast<long long>(kMostSlots - 2) * a.bt / kTile;
-  if (j.tiles_per_cta > most) j.tiles_per_cta = most < 1 ? 1 : static_cast<int>(most);
+  const Plan p = plan(a.n_sel, a.bt, a.kvh, resident(D));
+  j.total_tiles = p.total_tiles;
+  j.tiles_per_cta = p.tiles_per_cta;
   if (!a.lse_in) {
-    j.parts = (j.total_tiles + j.tiles_per_cta - 1) / j.tiles_per_cta;
+    j.parts = p.parts;
+    if (j.parts > a.parts_room) return cudaErrorInvalidValue;
     const cudaError_t e = launch_pass<BITS, D, LO, true>(j, s);
     if (e != cudaSuccess) return e;
   }

@@ -3,11 +3,13 @@ arguments of the rotary scalings at the edges of their ranges."""
 
 from __future__ import annotations
 
+import ctypes
 from types import SimpleNamespace
 
+import pytest
 import torch
 
-from kvssd_b200 import ops
+from kvssd_b200 import _native, ops
 
 CPU = torch.device("cpu")
 
@@ -30,3 +32,25 @@ def test_a_replaced_workspace_is_kept_with_its_status(monkeypatch):
     spaces.get(CPU, other, 100)
     assert len(spaces.status_words(None, 7)) == 2 and len(spaces.status_words(None)) == 3
     assert spaces.status_words(0) == []
+
+
+def weights_scratch(queries, places, qh, kvh, d, bits=4, group=32, bt=128):
+    need = ctypes.c_size_t()
+    _native.check(_native.library().kvssd_b200_attention_weights_scratch_size(
+        queries, -(-places // bt), bt, qh, kvh, d, bits, group, ctypes.byref(need)), "scratch size")
+    return need.value
+
+
+@pytest.mark.parametrize("d, group, bt", [(128, 32, 128), (256, 16, 16), (80, 16, 128), (64, 64, 1)])
+def test_weights_scratch_follows_what_is_used(d, group, bt):
+    """8 bytes a part and query row. The parts of a row: no more than there are tiles (of 32 places, of 16
+    for eight warps), and as many as come to 8 MB, or as four CTAs an SM shared by the KV heads, or as runs
+    of 510 blocks (of whole tiles of 128 places)."""
+    for kvh, places, queries in ((8, 131_072, 2048), (8, 1 << 20, 64), (1, 65_536, 32), (300, 5000, 3), (2, 40, 1)):
+        rows = queries * kvh * 4
+        parts, rest = divmod(weights_scratch(queries, places, 4 * kvh, kvh, d, group=group, bt=bt), 8 * rows)
+        assert rest == 0 and parts >= 1
+        blocks = -(-places // bt)
+        run = 128 * max(1, 510 * bt // 128)
+        assert parts <= max(1, 592 // kvh, (1 << 20) // rows, -(-blocks * bt // run))
+        assert parts <= max(-(-blocks * bt // 32), -(-blocks * -(-bt // 16) // 8))

@@ -13,6 +13,7 @@ import torch
 from kvssd_b200 import CacheSpec, DeviceBlockPool, DeviceKVCache, _native, ops
 from kvssd_b200.quant import quantize_tensor
 from oracle import cache_oracle as orc
+from test_gpu_cache_ops import check_weights
 
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda", 0)
@@ -102,6 +103,28 @@ def test_weights_nan_scores_show(shape):
     valid[-1] = bt - 1  # behind the valid rows it does not show
     out, lse = check_nan(clean, kp, broken, valid, bits, group, scale)
     assert not out.isnan().any() and not lse.isnan().any()
+
+
+@pytest.mark.parametrize("nb, bt, kvh, gqa, d, bits, group, queries, odd", [
+    (90, 40, 8, 1, 80, 4, 40, 2, False), (4000, 1, 2, 3, 32, 2, 8, 1, False), (60, 100, 4, 2, 36, 4, 12, 9, False),
+    (40, 128, 8, 2, 128, 4, 32, 3, True), (70, 100, 2, 20, 64, 2, 32, 2, True),
+    (3000, 1, 2, 40, 64, 4, 32, 1, False), (1500, 3, 1, 17, 96, 2, 32, 2, False), (2000, 2, 8, 2, 256, 2, 64, 30, False),
+    (700, 4, 160, 1, 64, 4, 32, 33, False), (300, 7, 8, 1, 128, 4, 16, 12, False), (5, 16, 600, 1, 80, 4, 16, 1, False),
+    (110, 40, 32, 1, 20, 4, 4, 256, False), (300, 16, 16, 1, 64, 4, 32, 512, True)])
+def test_weights_parts_of_the_log_sum_exps(nb, bt, kvh, gqa, d, bits, group, queries, odd):
+    """Computed log-sum-exps where blocks are so short that a CTA's run of places is, with more KV heads than
+    CTAs fit the GPU, and with so many rows that a CTA takes several runs; `odd`: a pool off 16 bytes."""
+    kp, ks = key_pool(nb, bt, kvh, d, bits, group, 8)
+    if odd:
+        far = torch.empty(kp.numel() + 1, dtype=torch.uint8, device=DEV)[1:].view(kp.shape)
+        kp = far.copy_(kp)
+    valid = torch.full((nb,), bt, dtype=torch.int32, device=DEV)
+    valid[-1] = 1
+    valid[nb // 3] = 0
+    query = torch.randn(queries, kvh * gqa, d, generator=gen(5)).half().to(DEV)
+    visible = (nb * bt - queries + 1 + torch.arange(queries)).int().to(DEV)
+    got = ops.attention_weights(query, kp, ks, valid, bits, group, 0.1, visible=visible)
+    check_weights(query, kp, ks, valid, bits, group, 0.1, visible=visible, got=got)
 
 
 # ------------------------------------------------------------------------------------------ append
