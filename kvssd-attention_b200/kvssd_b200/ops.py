@@ -767,7 +767,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, 
         _require_rows("out", out, x.shape, x.dtype, x.device)
         near, far = sorted(((out.stride(0), x.shape[0]), (out.stride(1), x.shape[1])))
         d = x.shape[2]
-        if (near[1] > 1 and near[0] < d) or (far[1] > 1 and far[0] < max(near[0] * near[1], d)):
+        if (near[1] > 1 and near[0] < d) or (far[1] > 1 and far[0] < near[0] * (near[1] - 1) + d):
             raise ValueError("out must not overlap itself")
     tokens, heads, d = x.shape
     kind = _INDEX_DTYPES.get(positions.dtype)

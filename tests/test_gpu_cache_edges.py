@@ -28,6 +28,37 @@ def key_pool(nb, bt, kvh, d, bits, group, seed):
     return q.packed.to(DEV), q.scales.to(DEV)
 
 
+# ------------------------------------------------------------------------------------------ rotary
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotary_into_views_that_leave_places_out(interleaved):
+    """Every second head of an odd number of heads, every second token, heads first: `out` does not overlap
+    itself, however close the rows lie; what lies between them stays."""
+    f = (10000.0 ** (-torch.arange(16, dtype=torch.float64) / 16)).to(DEV)
+    x = torch.randn(6, 5, 64, generator=gen(1)).half().to(DEV)
+    views = [lambda t: t[:, ::2], lambda t: t[::2], lambda t: t[::5, 1:4], lambda t: t[:1, ::4], lambda t: t[:, 2:3],
+             lambda t: t.transpose(0, 1)[::2], lambda t: t.view(30, 1, 64)[::29], lambda t: t.view(1, 30, 64)[:, ::29]]
+    for view in views:
+        want = view(x).contiguous()
+        positions = torch.arange(want.shape[0], device=DEV) + 9
+        want = ops.rotary(want, positions, f, interleaved=interleaved)
+        out = torch.full_like(x, 7.0)
+        assert ops.rotary(view(x), positions, f, interleaved=interleaved, out=view(out)).shape == want.shape
+        rest = out.clone()
+        view(rest).fill_(7.0)
+        assert torch.equal(view(out), want) and (rest == 7.0).all()
+        mine = x.clone()
+        ops.rotary(view(mine), positions, f, interleaved=interleaved, out=view(mine))
+        assert torch.equal(view(mine), want)
+    flat = torch.empty(600, dtype=torch.float16, device=DEV)
+    x = x[:2, :3]
+    positions = positions[:2]
+    for strides in ((64, 0), (0, 64), (63, 200), (200, 63), (191, 64), (64, 127), (128, 64)):
+        with pytest.raises(ValueError, match="overlap"):
+            ops.rotary(x, positions, f, out=flat.as_strided((2, 3, 64), (*strides, 1)))
+
+
 # ------------------------------------------------------------------------------- attention weights
 
 
