@@ -51,8 +51,8 @@ class RotaryEmbedding:
             raise ValueError("rotary_dim must be even and between 2 and head_dim")
         if self.scaling not in SCALINGS:
             raise ValueError(f"unknown scaling '{self.scaling}'; choose one of: {', '.join(SCALINGS)}")
-        if self.base <= 1.0 or self.factor < 1.0:
-            raise ValueError("base must be above 1 and factor at least 1")
+        if not 1.0 < self.base < math.inf or not 1.0 <= self.factor < math.inf:  # NaN: neither
+            raise ValueError("base must be above 1 and factor at least 1, both finite")
         if self.scaling == "ntk" and self.rotary_dim == 2:
             raise ValueError("ntk scaling needs a rotary_dim above 2")
         if self.scaling in ("smooth", "yarn"):
@@ -60,8 +60,8 @@ class RotaryEmbedding:
                 raise ValueError(f"{self.scaling} scaling needs the original_length")
             if self.high is None:
                 object.__setattr__(self, "high", 4.0 if self.scaling == "smooth" else 32.0)
-            if not 0 < self.low < self.high:
-                raise ValueError("low and high turns must be positive and ascending")
+            if not 0 < self.low < self.high < math.inf:
+                raise ValueError("low and high turns must be positive, ascending and finite")
 
     @property
     def magnitude(self) -> float:

@@ -4,12 +4,13 @@ arguments of the rotary scalings at the edges of their ranges."""
 from __future__ import annotations
 
 import ctypes
+import math
 from types import SimpleNamespace
 
 import pytest
 import torch
 
-from kvssd_b200 import _native, ops
+from kvssd_b200 import RotaryEmbedding, _native, ops
 
 CPU = torch.device("cpu")
 
@@ -54,3 +55,15 @@ def test_weights_scratch_follows_what_is_used(d, group, bt):
         run = 128 * max(1, 510 * bt // 128)
         assert parts <= max(1, 592 // kvh, (1 << 20) // rows, -(-blocks * bt // run))
         assert parts <= max(-(-blocks * bt // 32), -(-blocks * -(-bt // 16) // 8))
+
+
+@pytest.mark.parametrize("kw, text", [
+    (dict(base=math.nan), "base"), (dict(base=math.inf), "base"), (dict(scaling="linear", factor=math.nan), "factor"),
+    (dict(scaling="yarn", factor=math.inf, original_length=64), "factor"),
+    (dict(scaling="yarn", factor=2.0, original_length=64, high=math.inf), "finite"),
+    (dict(scaling="smooth", factor=2.0, original_length=64, low=math.nan), "ascending"),
+    (dict(scaling="smooth", factor=2.0, original_length=64, high=math.nan), "ascending")])
+def test_rotary_embedding_refuses_what_is_no_number(kw, text):
+    """They would make every frequency, and so every key, NaN without a word."""
+    with pytest.raises(ValueError, match=text):
+        RotaryEmbedding(128, **kw)
