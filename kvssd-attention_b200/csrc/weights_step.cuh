@@ -174,8 +174,9 @@ __global__ void __launch_bounds__(kThreads, step_resident(D, LO)) weights_step_k
       }
     }
     if (see <= 0) l2 = INFINITY;
+    if (l2 == INFINITY) see = 0;  // adds nothing, whatever a key's scale
     all_see = __reduce_min_sync(0xffffffffu, see > 0 ? see : 0x7fffffff);
-    if (all_see == 0x7fffffff && a.visible) all_see = 0;  // nothing is seen: mask every tile
+    if (!__any_sync(0xffffffffu, see > 0)) all_see = 0;  // nothing is seen: mask every tile
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       info[i].factor = __shfl_sync(0xffffffffu, q.factor, 4 * (2 * c + i)) * (BITS == 4 ? 1.f / kTiny : 1.f);

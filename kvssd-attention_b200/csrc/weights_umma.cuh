@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(threads(D), resident(D)) weights_umma_kernel(c
     const bool live = r < rows;
     const int t = live ? at / gqa : 0, head = h * gqa + (live ? at % gqa : 0);
     const long long q = (static_cast<long long>(t) * a.qh + head) * D;
-    const int n = !live ? 0 : a.visible ? a.visible[t] : 0x7fffffff;
+    int n = !live ? 0 : a.visible ? a.visible[t] : 0x7fffffff;
     const float given = a.lse_in && live ? a.lse_in[static_cast<long long>(t) * a.qh + head] : 0.f;
     float x[kMine][2][8] = {};
     float top = 0.f;
@@ -311,8 +311,9 @@ __global__ void __launch_bounds__(threads(D), resident(D)) weights_umma_kernel(c
       load_query8(a.query, a.dtype, q + 16 * unit, x[k][0]);
       load_query8(a.query, a.dtype, q + 16 * unit + 8, x[k][1]);
     }
-    // a row that adds nothing may hold anything (padding): it enters the products as zeros
+    // a row that adds nothing may hold anything (padding): it enters the products as zeros, and sees nothing
     const bool enters = n > 0 && given != -INFINITY;
+    if (!enters) n = 0;
 #pragma unroll
     for (int k = 0; k < kMine; ++k)
 #pragma unroll
@@ -440,10 +441,11 @@ __global__ void __launch_bounds__(threads(D), resident(D)) weights_umma_kernel(c
   float next_prev = mine_prev;
   load(1);
   int all_see = 0x7fffffff;  // places below are seen by every row that sees anything
+  bool any = false;
   for (int i = lane; i < rows; i += 32)
-    if (seen[i] > 0) all_see = min(all_see, seen[i]);
+    if (seen[i] > 0) all_see = min(all_see, seen[i]), any = true;
   all_see = __reduce_min_sync(0xffffffffu, all_see);
-  if (all_see == 0x7fffffff && a.visible) all_see = 0;
+  if (!__any_sync(0xffffffffu, any)) all_see = 0;
 
   const float own_factor = reinterpret_cast<const float*>(infos + row / 2)[row & 1];
   const int own_seen = seen[row];

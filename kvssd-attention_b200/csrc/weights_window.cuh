@@ -137,6 +137,7 @@ __global__ void __launch_bounds__(kThreads, resident(D, LO)) weights_tc_kernel(c
           v = as_log2(a.lse_in[to]);
         }
         if (n <= 0) v = INFINITY;
+        if (v == INFINITY) n = 0;  // adds nothing, whatever a key's scale
       }
     }
     if (lane == 0) {
@@ -145,10 +146,11 @@ __global__ void __launch_bounds__(kThreads, resident(D, LO)) weights_tc_kernel(c
     }
   }
   __syncthreads();
+  bool any = false;
   for (int i = lane; i < 8 * j.row_tiles; i += 32)
-    if (seen[i] > 0) all_see = min(all_see, seen[i]);
+    if (seen[i] > 0) all_see = min(all_see, seen[i]), any = true;
   all_see = __reduce_min_sync(0xffffffffu, all_see);
-  if (all_see == 0x7fffffff && a.visible) all_see = 0;  // nothing is seen: mask every tile
+  if (!__any_sync(0xffffffffu, any)) all_see = 0;  // nothing is seen: mask every tile
 
   // ---- the tiles
   float run_m[MODE == kLse ? 2 * kLseTiles : 1], run_l[MODE == kLse ? 2 * kLseTiles : 1];

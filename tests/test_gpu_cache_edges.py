@@ -136,6 +136,32 @@ def test_weights_nan_scores_show(shape):
     assert not out.isnan().any() and not lse.isnan().any()
 
 
+@pytest.mark.filterwarnings("ignore::RuntimeWarning")
+@pytest.mark.parametrize("shape", [*NAN_SHAPES, (80, 128, 2, 32, 2)])
+def test_weights_of_queries_that_add_nothing_beside_nan_keys(shape):
+    """Queries given as -inf add nothing to any place, to one whose key's scale is NaN neither; nor does
+    one that does not see that place."""
+    gqa, d, bits, group, queries = shape
+    kvh, nb, bt = 2, 5, 64
+    kp, ks = key_pool(nb, bt, kvh, d, bits, group, 3)
+    ks[2, 22, :, 0] = ks[4, 63] = math.nan
+    valid = torch.full((nb,), bt, dtype=torch.int32, device=DEV)
+    query = torch.randn(queries, kvh * gqa, d, generator=gen(4)).half().to(DEV)
+    previous = torch.rand(kvh, nb * bt, generator=gen(5)).to(DEV)
+    lse = torch.full((queries, kvh * gqa), -math.inf, device=DEV)
+    call = lambda **kw: ops.attention_weights(query, kp, ks, valid, bits, group, 0.1, lse=lse,  # noqa: E731
+                                              previous=previous, **kw)[0]
+    assert torch.equal(call(), previous)
+    lse[0, 0] = 3.0  # one row of KV head 0 that sees all
+    out = call()
+    assert torch.equal(out[1], previous[1])
+    assert out[0].isnan().nonzero().flatten().tolist() == [150, nb * bt - 1]
+    seen = torch.full((queries,), 150, dtype=torch.int32, device=DEV)  # one that sees the places before them
+    out = call(visible=seen)
+    assert torch.equal(out[1], previous[1]) and torch.equal(out[0, 150:], previous[0, 150:])
+    assert (out[0, :150] > previous[0, :150]).all()
+
+
 @pytest.mark.parametrize("nb, bt, kvh, gqa, d, bits, group, queries, odd", [
     (90, 40, 8, 1, 80, 4, 40, 2, False), (4000, 1, 2, 3, 32, 2, 8, 1, False), (60, 100, 4, 2, 36, 4, 12, 9, False),
     (40, 128, 8, 2, 128, 4, 32, 3, True), (70, 100, 2, 20, 64, 2, 32, 2, True),
