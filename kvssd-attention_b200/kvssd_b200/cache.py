@@ -175,10 +175,13 @@ class DeviceKVCache:
             return
         b = self.used_blocks
         ops.status_watch(self.device).poll("DeviceKVCache.evict (an earlier call)")
-        self.weights, self.positions = ops.evict(
-            self.weights, self.positions, self.n_tokens, keep, self.packed_k[:b], self.packed_v[:b],
-            self.scales_k[:b], self.scales_v[:b], self.valid_tokens[:b], sink=sink, recent=recent,
+        held = [t[:, :b * self.spec.block_tokens] for t in (self.weights, self.positions)]
+        new = ops.evict(
+            *held, self.n_tokens, keep, self.packed_k[:b], self.packed_v[:b], self.scales_k[:b],
+            self.scales_v[:b], self.valid_tokens[:b], sink=sink, recent=recent,
             next_position=self.next_position, shared=shared)
+        for t, of in zip(held, new):  # in place: a captured decode adds to these buffers
+            t.copy_(of)
         self.n_tokens = keep
         self._own_choices |= not shared
 

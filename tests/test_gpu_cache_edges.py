@@ -345,3 +345,32 @@ def test_a_graph_flags_in_a_workspace_that_has_been_replaced():
     graph.replay()
     assert ops.read_device_status_all(DEV) & _native.DEV_BAD_BLOCK
     assert ops.read_device_status_all(DEV) == 0
+
+
+def test_a_captured_decode_adds_to_the_weights_of_a_cache_that_evicted_since():
+    """The buffers of a cache stay where they are: a graph captured before an eviction reads and adds to
+    what the cache holds after it."""
+    cache = small_cache()
+    query = torch.randn(4, 64, generator=gen(3)).half().to(DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        cache.decode(query, observe=True)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        out, lse = cache.decode(query, observe=True)
+    torch.cuda.synchronize()
+    addresses = [t.data_ptr() for t in (cache.weights, cache.positions)]
+    cache.evict(5, sink=2, recent=1)
+    assert [t.data_ptr() for t in (cache.weights, cache.positions)] == addresses
+    assert (cache.weights[:, 5:] == 0).all() and (cache.positions[:, 5:] == -1).all()
+    assert (cache.positions[:, :5] >= 0).all()
+    before = cache.weights.clone()
+    graph.replay()
+    torch.cuda.synchronize()
+    added, own = ops.attention_weights(query, cache.packed_k, cache.scales_k, cache.valid_tokens, 4, 32, 1 / 8)
+    torch.testing.assert_close(cache.weights - before, added, rtol=1e-2, atol=1e-3)  # lse: the decode's
+    torch.testing.assert_close(lse, own, rtol=1e-3, atol=5e-3)
+    assert (cache.weights[:, 5:] == 0).all()
+    with torch.cuda.stream(side):
+        cache.check()
