@@ -25,7 +25,11 @@ class DeviceKVCache:
 
     ``n_tokens`` places are in use; place i is row i % block_tokens of block i // block_tokens.
     ``weights`` fp32 and ``positions`` int32 [kv_heads, places] hold each place's accumulated
-    attention weight and the position of the token that each KV head keeps there."""
+    attention weight and the position of the token that each KV head keeps there.
+
+    The counts live on the host. A captured ``decode`` or ``observe`` keeps the blocks and positions it
+    was captured with; ``append`` and ``evict``, which a replay would repeat on the same places, refuse
+    to be captured (a graph appends with ops.append, whose slots and positions lie on the device)."""
 
     def __init__(self, spec: CacheSpec, blocks: int, device: torch.device | str,
                  rotary: RotaryEmbedding | None = None):
@@ -85,6 +89,7 @@ class DeviceKVCache:
                values: bool = False) -> tuple[torch.Tensor, torch.Tensor] | None:
         """Adds the tokens of ``key`` and ``value`` [tokens, kv_heads, head_dim] (keys not yet rotated)
         at the next positions; see ops.append."""
+        self._not_captured("append")
         tokens = key.shape[0]
         n = self.n_tokens
         if n + tokens > self.capacity:
@@ -101,6 +106,10 @@ class DeviceKVCache:
         self.positions[:, n:n + tokens] = positions
         self.n_tokens, self.next_position = n + tokens, at + tokens
         return held
+
+    def _not_captured(self, call: str) -> None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"DeviceKVCache.{call} moves counts on the host and cannot be captured in a graph")
 
     def _in_use(self):
         if self.n_tokens == 0:
@@ -167,6 +176,7 @@ class DeviceKVCache:
         A cache that holds no more than ``keep`` tokens is left as it is. Once the heads have chosen
         for themselves, a shared choice has no meaning any more and is refused. A failure of an earlier
         call that is known by now is raised before anything moves; ``check()`` first waits for all."""
+        self._not_captured("evict")
         if keep < 1 or sink < 0 or recent < 0:
             raise ValueError("keep must be positive, sink and recent non-negative")
         if shared and self._own_choices:

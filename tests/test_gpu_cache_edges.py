@@ -374,3 +374,26 @@ def test_a_captured_decode_adds_to_the_weights_of_a_cache_that_evicted_since():
     assert (cache.weights[:, 5:] == 0).all()
     with torch.cuda.stream(side):
         cache.check()
+
+
+def test_cache_calls_that_move_counts_refuse_a_capture():
+    cache = small_cache()
+    x = torch.randn(1, 2, 64, generator=gen(3)).half().to(DEV)
+    query = torch.randn(4, 64, generator=gen(3)).half().to(DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ref = cache.decode(query)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        with pytest.raises(RuntimeError, match="cannot be captured"):
+            cache.append(x, x)
+        with pytest.raises(RuntimeError, match="cannot be captured"):
+            cache.evict(5)
+        out = cache.decode(query)
+    assert cache.n_tokens == cache.next_position == 13
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out[0], ref[0]) and torch.equal(out[1], ref[1])
+    cache.append(x, x)
+    assert cache.n_tokens == 14
