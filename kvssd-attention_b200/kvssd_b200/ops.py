@@ -392,6 +392,12 @@ def decode_combine(workspace: torch.Tensor, n_parts: int, query_heads: int, head
     return out, lse
 
 
+def _indexed(device: torch.device | str | None) -> torch.device:
+    """``device`` with its index: workspaces are kept by it. None, or no index: the current device."""
+    device = torch.device("cuda") if device is None else torch.device(device)
+    return torch.device("cuda", torch.cuda.current_device()) if device.index is None else device
+
+
 def read_device_status(device: torch.device | str | None = None, clear: bool = True,
                        stream: torch.cuda.Stream | None = None) -> int:
     """Synchronously reads the sticky device status word of the current (or given) stream's
@@ -403,7 +409,7 @@ def read_device_status(device: torch.device | str | None = None, clear: bool = T
     wait gave up (about a second) -- the out/lse of that call, and of later calls until the
     word is cleared, are NaN; bit 16: a batched problem descriptor was refused.
     """
-    device = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
+    device = _indexed(device)
     stream = stream or torch.cuda.current_stream(device)
     _workspaces.get(device, stream, _WORKSPACE_HEADER)
     return _read_words(device, _workspaces.status_words(device.index, stream.cuda_stream), clear, stream)
@@ -426,7 +432,7 @@ def _read_words(device: torch.device, workspaces: list[torch.Tensor], clear: boo
 def read_device_status_all(device: torch.device | str | None = None, clear: bool = True) -> int:
     """OR of the status words of every decode workspace on ``device`` (one per stream that has
     decoded, graph-capture streams included), read after synchronising the device."""
-    device = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
+    device = _indexed(device)
     torch.cuda.synchronize(device)
     return _read_words(device, _workspaces.status_words(device.index), clear,
                        torch.cuda.current_stream(device))
@@ -543,6 +549,7 @@ _watches: dict[tuple[int, int], _StatusWatch] = {}
 
 def status_watch(device: torch.device, stream: torch.cuda.Stream | None = None) -> _StatusWatch:
     """The status watch of ``device``'s current (or given) stream workspace."""
+    device = _indexed(device)
     stream = stream or torch.cuda.current_stream(device)
     key = (device.index, stream.cuda_stream)
     with _watch_lock:

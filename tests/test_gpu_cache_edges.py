@@ -397,3 +397,12 @@ def test_cache_calls_that_move_counts_refuse_a_capture():
     assert torch.equal(out[0], ref[0]) and torch.equal(out[1], ref[1])
     cache.append(x, x)
     assert cache.n_tokens == 14
+
+
+def test_status_of_a_device_given_without_its_index():
+    """"cuda" is the current device: its flags are found and cleared."""
+    ops.read_device_status(DEV)
+    for read in (ops.read_device_status, ops.read_device_status_all):
+        status_word().fill_(_native.DEV_BAD_BLOCK)
+        assert read("cuda") == _native.DEV_BAD_BLOCK and read("cuda") == 0 and read(DEV) == 0
+    assert ops.status_watch(torch.device("cuda")) is ops.status_watch(DEV)
