@@ -39,6 +39,7 @@ class _Workspaces:
         self._lock = threading.Lock()
         self._buffers: dict[tuple[int, int], torch.Tensor] = {}
         self._replaced: dict[tuple[int, int], list[torch.Tensor]] = {}
+        self._captured: set[tuple[int, int]] = set()  # zeroed by a graph, at each of its replays
 
     def get(self, device: torch.device, stream: torch.cuda.Stream, nbytes: int) -> torch.Tensor:
         key = (device.index, stream.cuda_stream)
@@ -49,12 +50,23 @@ class _Workspaces:
                 if buf is not None:
                     size = max(size, 2 * buf.numel())
                 old, buf = buf, torch.zeros(size, dtype=torch.uint8, device=device)
+                capturing = torch.cuda.is_current_stream_capturing()
                 if old is not None:
                     self._replaced.setdefault(key, []).append(old)
-                    if not torch.cuda.is_current_stream_capturing():
+                    if not capturing:
                         buf[:4].copy_(old[:4])  # what has been flagged and not been read
+                (self._captured.add if capturing else self._captured.discard)(key)
                 self._buffers[key] = buf
             return buf
+
+    def any_status_word(self, device_index: int) -> int | None:
+        """Address of a status word of the device that no graph clears, for a call captured on a stream
+        that has none (several streams' flags may share a word); None where nothing has run yet."""
+        with self._lock:
+            for key, buf in self._buffers.items():
+                if key[0] == device_index and key not in self._captured:
+                    return buf.data_ptr()
+        return None
 
     def status_words(self, device_index: int, stream: int | None = None) -> list[torch.Tensor]:
         """The workspaces of one stream (None: of every stream) of a device, replaced ones included:
@@ -431,7 +443,9 @@ def _read_words(device: torch.device, workspaces: list[torch.Tensor], clear: boo
 
 def read_device_status_all(device: torch.device | str | None = None, clear: bool = True) -> int:
     """OR of the status words of every decode workspace on ``device`` (one per stream that has
-    decoded, graph-capture streams included), read after synchronising the device."""
+    decoded, graph-capture streams included), read after synchronising the device. What a replayed graph
+    flags is found here: the cache-maintenance operators captured on a stream that has run nothing use
+    another stream's word."""
     device = _indexed(device)
     torch.cuda.synchronize(device)
     return _read_words(device, _workspaces.status_words(device.index), clear,
@@ -711,12 +725,12 @@ def _device_index(name: str, t: torch.Tensor) -> int:
 
 
 def _status_word(index: int, stream: int) -> int | None:
-    """Address of the stream's sticky status word (read_device_status, status_watch); None during a
-    graph capture on a stream that has none yet, since creating it would be captured."""
+    """Address of the stream's sticky status word (read_device_status, status_watch). Creating one during a
+    graph capture would be captured: another stream's serves then."""
     ws = _workspaces._buffers.get((index, stream))
     if ws is None:
         if torch.cuda.is_current_stream_capturing():
-            return None
+            return _workspaces.any_status_word(index)
         ws = _workspaces.get(torch.device("cuda", index), torch.cuda.current_stream(index),
                              _WORKSPACE_HEADER)
     return ws.data_ptr()

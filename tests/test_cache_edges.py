@@ -35,6 +35,20 @@ def test_a_replaced_workspace_is_kept_with_its_status(monkeypatch):
     assert spaces.status_words(0) == []
 
 
+def test_a_status_word_for_a_captured_call(monkeypatch):
+    """A stream without a workspace borrows a word that no graph clears."""
+    spaces = ops._Workspaces()
+    capturing = True
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing)
+    in_graph, eager = SimpleNamespace(cuda_stream=7), SimpleNamespace(cuda_stream=8)
+    assert spaces.any_status_word(None) is None
+    spaces.get(CPU, in_graph, 100)
+    assert spaces.any_status_word(None) is None
+    capturing = False
+    buf = spaces.get(CPU, eager, 100)
+    assert spaces.any_status_word(None) == buf.data_ptr() and spaces.any_status_word(0) is None
+
+
 def weights_scratch(queries, places, qh, kvh, d, bits=4, group=32, bt=128):
     need = ctypes.c_size_t()
     _native.check(_native.library().kvssd_b200_attention_weights_scratch_size(

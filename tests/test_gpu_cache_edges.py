@@ -406,3 +406,25 @@ def test_status_of_a_device_given_without_its_index():
         status_word().fill_(_native.DEV_BAD_BLOCK)
         assert read("cuda") == _native.DEV_BAD_BLOCK and read("cuda") == 0 and read(DEV) == 0
     assert ops.status_watch(torch.device("cuda")) is ops.status_watch(DEV)
+
+
+def test_a_graph_of_a_fresh_stream_flags_what_it_refuses():
+    """Captured on the stream that a graph brings along, which has run nothing: a slot behind the pool is
+    reported all the same, of every replay."""
+    pool = [torch.zeros(2, 4, 1, 16, dtype=torch.uint8, device=DEV) for _ in "kv"] + [
+        torch.zeros(2, 4, 1, 1, dtype=torch.float16, device=DEV) for _ in "kv"]
+    x = torch.randn(2, 1, 32, generator=gen(1)).to(DEV)
+    slots = torch.tensor([1, 3], device=DEV)
+    ops.append(x, x, slots, *pool, 4, 32)  # elsewhere
+    torch.cuda.synchronize()
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=stream):
+        ops.append(x, x, slots, *pool, 4, 32)
+    assert ops.read_device_status_all(DEV) == 0
+    graph.replay()
+    assert ops.read_device_status_all(DEV) == 0
+    slots[1] = 8
+    for _ in range(2):
+        graph.replay()
+        assert ops.read_device_status_all(DEV) == _native.DEV_BAD_BLOCK
+    assert ops.read_device_status_all(DEV) == 0
