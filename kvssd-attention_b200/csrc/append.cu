@@ -249,7 +249,7 @@ constexpr int resident(int iters, int bytes, bool turns) {
 
 template <typename T, int BITS, bool INTERLEAVED, int kIters, int kGroupLanes, bool TURNS>
 __global__ void __launch_bounds__(kThreads, resident(kIters, sizeof(T), TURNS))
-    append_rows_kernel(const AppendArgs a, int chunks, unsigned per_lane, int heads, int per_warp, int kv0) {
+    append_rows_kernel(const AppendArgs a, unsigned per_lane, int heads, int per_warp) {
   extern __shared__ Turn turns[];  // [warps][per_warp][pairs]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int lanes = a.d >> 3;                                   // of a row
@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(kThreads, resident(kIters, sizeof(T), TURNS))
   const int step = kIters == 1 ? heads : 32u * per_lane >> 16;  // several steps use all of a warp's rows
   const int tokens = kIters == 1 ? per_warp : 1;  // of the warp
   const int nth = kIters == 1 ? row / step : 0, step_row = row - nth * step;
-  const int later = static_cast<int>(blockIdx.y) >= chunks, kv = kv0 + later, chunk = blockIdx.y - later * chunks;
+  const int kv = blockIdx.y & 1, chunk = blockIdx.y >> 1;
   const int token0 = (blockIdx.x * (kThreads / 32) + warp) * tokens, token = token0 + nth;
   const int pairs = a.freq ? a.pairs : 0;
   pdl_wait();
@@ -388,25 +388,23 @@ __global__ void __launch_bounds__(kThreads, resident(kIters, sizeof(T), TURNS))
 }
 
 template <typename T, int BITS, bool INTERLEAVED, int kIters>
-cudaError_t launch_iters(const AppendArgs& a, int step, int per_warp, bool few, cudaStream_t s) {
+cudaError_t launch_iters(const AppendArgs& a, int step, int per_warp, cudaStream_t s) {
   const int warps = kThreads / 32, chunks = (a.kvh + kIters * step - 1) / (kIters * step);
   // lane / lanes as a product: 2^16 / lanes rounded up is exact for 32 lanes
   const unsigned per_lane = (65536u + a.d / 8 - 1) / (a.d / 8);
-  const dim3 both((a.tokens + warps * per_warp - 1) / (warps * per_warp), 2 * chunks), one(both.x, chunks);
-  const size_t smem = a.freq ? static_cast<size_t>(warps) * per_warp * a.pairs * sizeof(Turn) : 0;
+  const dim3 grid((a.tokens + warps * per_warp - 1) / (warps * per_warp), 2 * chunks);
   const bool g32 = a.group == 32;
-  const auto turned = g32 ? append_rows_kernel<T, BITS, INTERLEAVED, kIters, 4, true>
-                          : append_rows_kernel<T, BITS, INTERLEAVED, kIters, 0, true>;
-  if (few) return launch_pdl(turned, both, kThreads, smem, s, a, chunks, per_lane, step, per_warp, 0);
-  // Many tokens: values (and keys that do not turn) in a launch of their own, which needs half the
-  // registers (8192 tokens that do not turn: 14.8 us, by the kernel that can turn 18.5; keys that turn make
-  // the two launches 26.8 us, in one 26.4).
-  const auto plain = g32 ? append_rows_kernel<T, BITS, false, kIters, 4, false>
-                         : append_rows_kernel<T, BITS, false, kIters, 0, false>;
-  const cudaError_t e = launch_pdl(plain, a.freq ? one : both, kThreads, 0, s, a, chunks, per_lane, step, per_warp,
-                                   a.freq ? 1 : 0);
-  if (e != cudaSuccess || !a.freq) return e;
-  return launch_pdl(turned, one, kThreads, smem, s, a, chunks, per_lane, step, per_warp, 0);
+  // Keys that do not turn take the kernel that needs half the registers (8192 tokens: 14.8 us, by the kernel
+  // that can turn 18.5). Where they do turn, values in a launch of their own are no faster (25.8 us for
+  // 25.1; 2048 tokens 13.1 for 8.9).
+  if (!a.freq)
+    return launch_pdl(g32 ? append_rows_kernel<T, BITS, false, kIters, 4, false>
+                          : append_rows_kernel<T, BITS, false, kIters, 0, false>,
+                      grid, kThreads, 0, s, a, per_lane, step, per_warp);
+  const size_t smem = static_cast<size_t>(warps) * per_warp * a.pairs * sizeof(Turn);
+  return launch_pdl(g32 ? append_rows_kernel<T, BITS, INTERLEAVED, kIters, 4, true>
+                        : append_rows_kernel<T, BITS, INTERLEAVED, kIters, 0, true>,
+                    grid, kThreads, smem, s, a, per_lane, step, per_warp);
 }
 
 template <typename T, int BITS, bool INTERLEAVED>
@@ -416,10 +414,10 @@ cudaError_t launch_rows(const AppendArgs& a, cudaStream_t s) {
   // one step a task spreads the work over more warps instead.
   const int rows = 32 / (a.d / 8), step = rows < a.kvh ? rows : a.kvh, steps = (a.kvh + step - 1) / step;
   const bool few = 2ll * a.tokens * ((steps + 3) / 4) < 148 * 16;
-  if (few) return launch_iters<T, BITS, INTERLEAVED, 1>(a, step, 1, true, s);
-  if (steps == 1) return launch_iters<T, BITS, INTERLEAVED, 1>(a, step, rows / step, false, s);
-  if (steps == 2) return launch_iters<T, BITS, INTERLEAVED, 2>(a, step, 1, false, s);
-  return launch_iters<T, BITS, INTERLEAVED, 4>(a, step, 1, false, s);
+  if (few) return launch_iters<T, BITS, INTERLEAVED, 1>(a, step, 1, s);
+  if (steps == 1) return launch_iters<T, BITS, INTERLEAVED, 1>(a, step, rows / step, s);
+  if (steps == 2) return launch_iters<T, BITS, INTERLEAVED, 2>(a, step, 1, s);
+  return launch_iters<T, BITS, INTERLEAVED, 4>(a, step, 1, s);
 }
 
 // Whether append_rows_kernel takes this call.
