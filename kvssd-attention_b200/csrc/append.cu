@@ -410,10 +410,12 @@ cudaError_t launch_iters(const AppendArgs& a, int step, int per_warp, cudaStream
 template <typename T, int BITS, bool INTERLEAVED>
 cudaError_t launch_rows(const AppendArgs& a, cudaStream_t s) {
   // Heads a warp takes at a time, and steps to take them all. Up to four steps a task keep 2 KB a warp in
-  // flight, no more than there are heads for (4 heads of 128: two steps 30.2 us, four 39.7); with few tokens
-  // one step a task spreads the work over more warps instead.
+  // flight, no more than there are heads for (4 heads of 128: two steps 30.2 us, four 39.7). One step a task
+  // spreads the work of few tokens over more warps: up to 32 an SM (8 heads of 128, 128 tokens: one step
+  // 3.4 us, four 4.7; 450: 4.7 both; 1100: 7.8 and 6.6. One head of 64, 600 tokens: 3.1 us, four tokens a
+  // warp 3.9; 2400: 4.9 and 4.7).
   const int rows = 32 / (a.d / 8), step = rows < a.kvh ? rows : a.kvh, steps = (a.kvh + step - 1) / step;
-  const bool few = 2ll * a.tokens * ((steps + 3) / 4) < 148 * 16;
+  const bool few = 2ll * a.tokens * steps < 148 * 32;
   if (few) return launch_iters<T, BITS, INTERLEAVED, 1>(a, step, 1, s);
   if (steps == 1) return launch_iters<T, BITS, INTERLEAVED, 1>(a, step, rows / step, s);
   if (steps == 2) return launch_iters<T, BITS, INTERLEAVED, 2>(a, step, 1, s);
