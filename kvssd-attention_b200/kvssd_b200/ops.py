@@ -503,19 +503,22 @@ class _StatusWatch:
 
     def __init__(self, device: torch.device, stream: torch.cuda.Stream):
         self.device, self.stream = device, stream
-        self._host = torch.zeros(self.SLOTS, dtype=torch.int32, pin_memory=True)
-        self._events: list[torch.cuda.Event | None] = [None] * self.SLOTS
+        self._host = list(torch.zeros(self.SLOTS, dtype=torch.int32, pin_memory=True).split(1))
+        self._own_events = [torch.cuda.Event() for _ in range(self.SLOTS)]
+        self._events: list[torch.cuda.Event | None] = [None] * self.SLOTS  # those of outstanding reads
+        self._word: tuple[torch.Tensor, torch.Tensor] | None = None  # the workspace and its status word
         self._next = 0
 
     def _take(self, i: int, block: bool) -> int:
         ev = self._events[i]
         if ev is None:
             return 0
-        if not block and not ev.query():
-            return 0
-        ev.synchronize()
+        if not ev.query():
+            if not block:
+                return 0
+            ev.synchronize()
         self._events[i] = None
-        return int(self._host[i])
+        return self._host[i].item()
 
     def _raise(self, value: int, where: str) -> None:
         if value & FAILURE_BITS:
@@ -530,11 +533,15 @@ class _StatusWatch:
         i = self._next % self.SLOTS
         self._raise(self._take(i, block=True), where)  # the slot's earlier read, long done
         ws = _workspaces.get(self.device, self.stream, _WORKSPACE_HEADER)
-        with torch.cuda.stream(self.stream):
-            self._host[i:i + 1].copy_(ws[:4].view(torch.int32), non_blocking=True)
-        ev = torch.cuda.Event()
-        ev.record(self.stream)
-        self._events[i] = ev
+        if self._word is None or self._word[0] is not ws:
+            self._word = ws, ws[:4].view(torch.int32)
+        if _raw_stream(self.device.index) == self.stream.cuda_stream:
+            self._host[i].copy_(self._word[1], non_blocking=True)
+        else:
+            with torch.cuda.stream(self.stream):
+                self._host[i].copy_(self._word[1], non_blocking=True)
+        self._own_events[i].record(self.stream)
+        self._events[i] = self._own_events[i]
         self._next += 1
 
     def poll(self, where: str) -> None:
@@ -563,7 +570,8 @@ _watches: dict[tuple[int, int], _StatusWatch] = {}
 
 def status_watch(device: torch.device, stream: torch.cuda.Stream | None = None) -> _StatusWatch:
     """The status watch of ``device``'s current (or given) stream workspace."""
-    device = _indexed(device)
+    if device.index is None:
+        device = _indexed(device)
     stream = stream or torch.cuda.current_stream(device)
     key = (device.index, stream.cuda_stream)
     with _watch_lock:
