@@ -52,9 +52,10 @@ class DeviceKVCache:
         self.scales_k = torch.zeros(scales, dtype=torch.float16, device=device)
         self.scales_v = torch.zeros(scales, dtype=torch.float16, device=device)
         self.valid_tokens = torch.zeros(blocks, dtype=torch.int32, device=device)
-        self.weights = torch.zeros((spec.kv_heads, self.capacity), dtype=torch.float32, device=device)
-        self.positions = torch.full((spec.kv_heads, self.capacity), -1, dtype=torch.int32,
-                                    device=device)
+        # one buffer, so that what an eviction leaves is copied back at once; a second one at the first
+        self._stats = [torch.zeros((2, spec.kv_heads, self.capacity), dtype=torch.int32, device=device)]
+        self._weights, self._positions = self._parts(self._stats[0])
+        self._positions.fill_(-1)
         self._places = torch.arange(self.capacity, dtype=torch.int32, device=device)
         self.n_tokens = 0
         self.next_position = 0
@@ -76,6 +77,18 @@ class DeviceKVCache:
         cache.positions[:, :n_tokens] = cache._places[:n_tokens]
         cache.n_tokens = cache.next_position = n_tokens
         return cache
+
+    @staticmethod
+    def _parts(stats: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        return stats[0].view(torch.float32), stats[1]
+
+    @property
+    def weights(self) -> torch.Tensor:
+        return self._weights
+
+    @property
+    def positions(self) -> torch.Tensor:
+        return self._positions
 
     @property
     def capacity(self) -> int:
@@ -185,13 +198,14 @@ class DeviceKVCache:
             return
         b = self.used_blocks
         ops.status_watch(self.device).poll("DeviceKVCache.evict (an earlier call)")
-        held = [t[:, :b * self.spec.block_tokens] for t in (self.weights, self.positions)]
-        new = ops.evict(
-            *held, self.n_tokens, keep, self.packed_k[:b], self.packed_v[:b], self.scales_k[:b],
-            self.scales_v[:b], self.valid_tokens[:b], sink=sink, recent=recent,
-            next_position=self.next_position, shared=shared)
-        for t, of in zip(held, new):  # in place: a captured decode adds to these buffers
-            t.copy_(of)
+        if len(self._stats) == 1:
+            self._stats.append(torch.empty_like(self._stats[0]))
+            self._evicted = self._parts(self._stats[1])
+        ops.evict(
+            self.weights, self.positions, self.n_tokens, keep, self.packed_k[:b], self.packed_v[:b],
+            self.scales_k[:b], self.scales_v[:b], self.valid_tokens[:b], sink=sink, recent=recent,
+            next_position=self.next_position, shared=shared, out=self._evicted)
+        self._stats[0].copy_(self._stats[1])  # in place: a captured decode adds to these buffers
         self.n_tokens = keep
         self._own_choices |= not shared
 

@@ -1027,11 +1027,11 @@ def evict(weights: torch.Tensor, positions: torch.Tensor, n_tokens: int, keep: i
           packed_k: torch.Tensor, packed_v: torch.Tensor, scales_k: torch.Tensor,
           scales_v: torch.Tensor, valid_tokens: torch.Tensor, *,
           block_table: torch.Tensor | None = None, sink: int = 0, recent: int = 0,
-          next_position: int | None = None,
-          shared: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+          next_position: int | None = None, shared: bool = False,
+          out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Compacts a cache of ``n_tokens`` tokens in place to the ``keep`` tokens of the largest
     accumulated weight; returns (weights, positions) of the compacted cache, shaped as given, 0 and -1
-    from ``keep`` on.
+    from ``keep`` on: in new tensors or in those of ``out`` (contiguous; they must not overlap the inputs).
 
     Place i of the cache is row i % block_tokens of the i // block_tokens-th selected block
     (``block_table`` entries must differ; None: the pool in order); its blocks before the last hold
@@ -1079,8 +1079,17 @@ def evict(weights: torch.Tensor, positions: torch.Tensor, n_tokens: int, keep: i
     end = n_tokens if next_position is None else next_position
     recent_from = end - recent if recent else 1 << 40  # behind every position
     lists = 1 if shared else kvh
-    new_weights = torch.empty((kvh, columns), dtype=torch.float32, device=weights.device)
-    new_positions = torch.empty((kvh, columns), dtype=torch.int32, device=weights.device)
+    if out is None:
+        new_weights = torch.empty((kvh, columns), dtype=torch.float32, device=weights.device)
+        new_positions = torch.empty((kvh, columns), dtype=torch.int32, device=weights.device)
+    else:
+        new_weights, new_positions = out
+        for name, t, dtype in (("out[0]", new_weights, torch.float32), ("out[1]", new_positions, torch.int32)):
+            _require_cuda(name, t, weights.device, dtype)
+            if t.shape != (kvh, columns):
+                raise ValueError(f"{name} must be [{kvh}, {columns}], got {tuple(t.shape)}")
+            if t.data_ptr() in (weights.data_ptr(), positions.data_ptr()):
+                raise ValueError("out must not overlap weights or positions")
     ints = lists * (n_tokens + 1)
     if n_tokens > 1 << 17:  # the longest caches need more
         need = ctypes.c_size_t()

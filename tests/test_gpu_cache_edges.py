@@ -243,6 +243,30 @@ def test_append_with_a_magnitude(tokens, kvh, d, bits, group, pairs, dtype, inte
         assert torch.equal(pool[2 + i].flatten(0, 1)[:tokens].cpu(), q.scales)
 
 
+# ------------------------------------------------------------------------------------------- evict
+
+
+def test_evict_into_given_tensors():
+    weights = torch.rand(2, 40, generator=gen(1)).to(DEV)
+    positions = torch.arange(40, dtype=torch.int32, device=DEV).expand(2, 40).contiguous()
+    pool = [torch.randint(0, 256, (5, 8, 2, 16), generator=gen(2), dtype=torch.uint8).to(DEV) for _ in "kv"] + [
+        torch.rand(5, 8, 2, 1, generator=gen(3)).half().to(DEV) for _ in "kv"]
+    call = lambda out=None: ops.evict(weights, positions, 37, 20, *(t.clone() for t in pool),  # noqa: E731
+                                      torch.zeros(5, dtype=torch.int32, device=DEV), sink=2, out=out)
+    want = call()
+    wide = torch.full((4, 2, 40), 9, dtype=torch.int32, device=DEV)
+    out = wide[1].view(torch.float32), wide[2]
+    got = call(out)
+    assert got[0] is out[0] and got[1] is out[1]
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert (wide[0] == 9).all() and (wide[3] == 9).all()
+    spare = torch.empty_like(weights), torch.empty_like(positions)
+    for bad in ((weights, spare[1]), (spare[0], positions), (spare[0].double(), spare[1]), (spare[0], spare[1].long()),
+                (spare[0][:, :39], spare[1]), (spare[0], spare[1][:1]), (spare[0].cpu(), spare[1])):
+        with pytest.raises(ValueError):
+            call(bad)
+
+
 # ------------------------------------------------------------------------------------ DeviceKVCache
 
 
