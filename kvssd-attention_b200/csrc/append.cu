@@ -11,8 +11,9 @@
 // By its bytes bound by HBM: the inputs are read once, codes and scales (and, when asked for, the FP16
 // values that the codes stand for) are written once. The arithmetic comes close to that time, so it works
 // on two elements an instruction and divides by remainders. 8192 tokens x 8 heads x 128 BF16 to INT4:
-// 14.8 us with the values written (floor 11.7), 12.1 without; keys rotated 26.8 and 23.0, bound by the
-// latency of the rotation's chain at the 16 to 24 warps an SM that its registers leave.
+// 15.2 us with the values written (floor 11.7); keys rotated 25.7 (FP32 keys 32.0, floor 16.8), bound by the
+// latency of the rotation's chain at the 16 to 24 warps an SM that its registers leave (58 % of the issue
+// slots are used; the four-step form of 16-bit types spills 12 bytes a thread at its 80 registers).
 //
 // append_rows_kernel: scale groups and pairs of whole 8 elements, rows on 16 bytes. append_kernel is
 // the form for any other shape and alignment: a CTA takes one token, a warp one scale group after the
@@ -238,7 +239,7 @@ struct alignas(16) Eight {
 // A lane holds 8 consecutive elements of a row (head), a row is d / 8 lanes, a warp takes `heads` rows at a
 // time; a task is kIters such steps over the heads of one token's keys or values, their loads all in flight
 // at once. Where one step takes all heads and leaves half of a warp's lanes or more without work, a task is
-// that step of `per_warp` tokens (8.4 M elements, one head of 64: 63 us, with one token a warp 244). The cos
+// that step of `per_warp` tokens (8.4 M elements, one head of 64: 59 us, with one token a warp 244). The cos
 // and sin of a token's pairs are computed by the task's lanes and handed around through shared memory, then
 // stay in registers over the heads; a rotation's other element comes from a lane of the same row (half
 // layout) or is the lane's own (interleaved). kGroupLanes: the lanes of a scale group, 0: any number.
@@ -395,8 +396,8 @@ cudaError_t launch_iters(const AppendArgs& a, int step, int per_warp, cudaStream
   const dim3 grid((a.tokens + warps * per_warp - 1) / (warps * per_warp), 2 * chunks);
   const bool g32 = a.group == 32;
   // Keys that do not turn take the kernel that needs half the registers (8192 tokens: 14.8 us, by the kernel
-  // that can turn 18.5). Where they do turn, values in a launch of their own are no faster (25.8 us for
-  // 25.1; 2048 tokens 13.1 for 8.9).
+  // that can turn 18.5). Where they do turn, values in a launch of their own are slower (25.9 us for 24.6;
+  // 2048 tokens 13.1 for 8.8).
   if (!a.freq)
     return launch_pdl(g32 ? append_rows_kernel<T, BITS, false, kIters, 4, false>
                           : append_rows_kernel<T, BITS, false, kIters, 0, false>,

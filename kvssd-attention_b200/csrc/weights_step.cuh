@@ -9,9 +9,10 @@
 // round at the size of that start, which is the size of the codes' own sum. INT2 codes are mostly
 // zero, their sums far below such a start, so they are centred first (half as many bytes to unpack).
 //
-// One step of 8 KV heads x 4 query heads x 128: 131072 tokens INT4 20.8 us, 0.61 of the measured copy
-// rate (84 MB; about 5 us are the start, the rest runs at 0.77 of that rate, bound by issuing about
-// 310 instructions a 32-place tile); INT2 23.2 us; 8192 tokens 5.5 us, all of it start. Tiles of 16
+// One step of 8 KV heads x 4 query heads x 128: 131072 tokens INT4 21.4 us, 0.60 of the measured copy
+// rate (84 MB; about 5 us are the start, the rest runs at 0.78 of that rate, bound by issuing: 355
+// instructions a 32-place tile, the start's included, in half of all issue slots at 16 warps an SM); INT2
+// 22.3 us (398 instructions); 8192 tokens 6.2 us, all of it start. FP32 queries 29 us. Tiles of 16
 // places with three or four CTAs an SM took 28 to 36 us.
 #pragma once
 
@@ -23,6 +24,8 @@ namespace weights_tc {
 constexpr int kStepStages = 3;
 constexpr float kTiny = 5.9604644775390625e-8f;  // 2^-24, FP16's smallest subnormal
 constexpr int step_rows(int d, int unit, bool lo) { return d <= 128 && unit == 32 && !lo ? 32 : 16; }
+// Resident CTAs to leave registers for. Units of 16 dims at head_dim 256 spill about 0.5 KB a thread at two
+// (131072 places x 4 heads INT4 in groups of 16: 57 us).
 constexpr int step_resident(int d, bool lo) { return d == 256 && lo ? 1 : 2; }
 
 // Codes of one lane, row and unit: INT4 as pairs n 2^-24 2^step_shift(p), INT2 centred.

@@ -2,13 +2,14 @@
 // scale groups of whole 16 dims.
 //
 // Math. A warp takes tiles of 16 (or 32) places of one KV head: S = K Q^T with mma.sync m16n8k16,
-// 16 places by 8 query rows. The codes enter as exact centred FP16 integers and the queries as FP16
-// (FP32 and FP64 ones as a high and a low part), each row scaled by a power of two to the top of
-// FP16's range, so that every product is exact and the FP32 sums are the only rounding; the FP16 key
-// scales are constant over a unit of 32 (or 16) dims and multiply the unit's partial sums in FP32.
+// 16 places by 8 query rows. The codes enter as exact centred FP16 integers and the queries as FP16, each
+// row scaled by a power of two to the top of FP16's range: FP16 and BF16 ones as they are but for a rounding
+// at 2^-39 of the row's largest, FP32 and FP64 ones as a high and a low part, 22 bits. Products are exact
+// then and sums FP32; the FP16 key scales are constant over a unit of 32 (or 16) dims and multiply the
+// unit's partial sums in FP32. Exponentials are ex2.approx, log-sum-exps pass through base 2 in FP32.
 // More than 32 rows go to tcgen05 (weights_umma.cuh): its tiles are 128 rows wide however few are used.
-// 65536 tokens x 8 heads x 128 INT4, log-sum-exps computed: 16 rows 54 us and 32 rows 70 us here, 64 rows
-// 99 us and 128 rows 112 us there.
+// 65536 tokens x 8 heads x 128 INT4, log-sum-exps computed: 16 rows 52 us and 32 rows 69 us here, 64 rows
+// 103 us and 128 rows 118 us there.
 //
 // Unit layout. A lane (r, c) of the A fragment holds the codes of row r (and r + 8) that lie c-th of
 // four in the unit: 8 codes of a 32-dim unit, 4 of a 16-dim unit, unpacked two at a time into pairs

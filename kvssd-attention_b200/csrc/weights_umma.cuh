@@ -5,9 +5,12 @@
 // as FP16: a centred INT2 code times its FP16 scale is exact in FP16; an INT4 one has up to 14 bits and
 // goes in as two FP16 terms, hi = RN(code * scale) and lo = code * scale - hi, which is exact. Queries
 // are FP16 (FP32 and FP64 ones a high and a low part), each row brought to the top of FP16's range by a
-// power of two. So tcgen05.mma's FP32 sums are the only rounding, and no scale is applied behind them.
+// power of two (what that rounds is said in weights_tc.cuh). Of two keys' terms and two queries' the product
+// of the low ones, 2^-22 of the whole, is left out. No scale is applied behind tcgen05.mma's FP32 sums.
 // Scales so large that a product leaves FP16's range (above 8188, or 32752 at INT2) are divided by 16
-// for the whole tile, whose scores are multiplied by 16 again.
+// for the whole tile, whose scores are multiplied by 16 again (scales below 2^-10 beside them are
+// rounded to FP16's subnormals then: an element of such a key is off by up to 2^-18, where one of the large
+// scale's is a multiple of 2^13).
 //
 // Two passes: the log-sum-exps put the queries on the accumulator's lanes and the places on its columns
 // (a thread keeps the running max and sum of its query row), the weights the other way round (a thread
@@ -16,11 +19,13 @@
 //
 // A CTA walks a run of tiles: it waits for the MMAs of tile i, unpacks tile i + 1 into the one key buffer,
 // issues its MMAs into the other half of the accumulator, and works on tile i's scores while they run. Two
-// CTAs share an SM (one of twice the threads at head_dim 256). Codes are loaded a tile ahead into registers.
+// CTAs share an SM (one of twice the threads at head_dim 256; one where INT4 keys and FP32 queries, in two
+// terms each, fill its shared memory). Codes are loaded a tile ahead into registers.
 //
-// 65536 tokens x 8 heads x 128 INT2, 32 queries x 4 query heads, both passes: 88 us, of which 30 are
-// exponentials; a tile takes a CTA about 3700 clocks (log-sum-exps) and 5100 (weights), unpacking and the
-// barriers' turns beside the exponentials, and a pass about 4.5 us to start. INT4: 112 us.
+// 65536 tokens x 8 heads x 128 INT2, 32 queries x 4 query heads, both passes: 91 us, of which 30 are
+// exponentials; a CTA's run of 14 tiles takes 83 thousand clocks (log-sum-exps) and 105 thousand (weights)
+// from a cold cache, 5900 and 7500 a tile with the start: unpacking and the barriers' turns beside the
+// exponentials. INT4: 118 us. FP32 queries: INT2 103 us, INT4 168 us.
 #pragma once
 
 #include "tma.cuh"

@@ -775,12 +775,13 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, 
            interleaved: bool = False, magnitude: float = 1.0,
            out: torch.Tensor | None = None) -> torch.Tensor:
     """Rotary positions of ``x`` [tokens, heads, head_dim] (FP32, FP16 or BF16; any token and head
-    strides), in a new tensor or in ``out``, which may be ``x`` itself.
+    strides), in a new tensor or in ``out``, which may be ``x`` itself and else must not overlap it.
 
     ``positions`` int32 or int64 [tokens]; ``frequencies`` float64 [pairs], radians a position (see
     rotary.RotaryEmbedding for the usual scalings). The first 2 * pairs dims of a head are rotated
     -- pair i is dims (i, i + pairs), or (2i, 2i + 1) when ``interleaved`` --, the dims behind are
-    copied. Angles are FP64, products FP32, rounded once."""
+    copied. Angles are FP64; cos and sin, the ``magnitude`` that multiplies them and the products FP32,
+    rounded once."""
     index = _device_index("rotary", x)
     dtype = _ELEMENT_DTYPES.get(x.dtype)
     if dtype is None:
@@ -851,7 +852,7 @@ def append(key: torch.Tensor, value: torch.Tensor, slots: torch.Tensor, packed_k
     (padding), one behind the pool is skipped and flagged (read_device_status bit 1). The slots of
     one call must differ from each other. With ``frequencies`` and ``positions`` the keys are rotated
     first (as ``rotary``, but rounded to FP32 once instead of to their type). Codes and scales equal
-    quant.quantize_tensor's bit for bit. ``valid_tokens`` (optional): the counts of the written
+    quant.quantize_tensor's bit for bit, except the codes of groups that hold a NaN or an infinity. ``valid_tokens`` (optional): the counts of the written
     blocks are raised to cover the written rows. ``values=True`` returns the FP16 keys and values that
     the cache now holds for the tokens ([tokens, kv_heads, head_dim], skipped tokens included), for a
     prompt's own attention to see what later decodes will see."""
@@ -951,7 +952,7 @@ def attention_weights(query: torch.Tensor, packed_k: torch.Tensor, scales_k: tor
     counts for query t when its row lies before the block's valid count and i < ``visible``[t] (int32
     [queries]; None: all). ``lse`` fp32 [query_heads] or [queries, query_heads]: as ``decode``
     returned it for these queries, or None to compute it (a first pass over the keys). ``out`` may be
-    ``previous``. The returned lse is -inf for a query that sees nothing; it adds nothing."""
+    ``previous`` and else must not overlap it. The returned lse is -inf for a query that sees nothing; it adds nothing."""
     index = _device_index("attention_weights", query)
     dtype = _QUERY_DTYPES.get(query.dtype)
     if dtype is None:
