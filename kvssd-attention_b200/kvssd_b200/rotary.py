@@ -90,7 +90,8 @@ class RotaryEmbedding:
         return freq
 
     def on(self, device: torch.device | str) -> torch.Tensor:
-        """``frequencies()`` on ``device``, kept there for later calls."""
+        """``frequencies()`` on ``device``, kept there for later calls. The first call on a device copies
+        them, which cannot be captured in a graph."""
         device = torch.device(device)
         if device.type == "cuda" and device.index is None:
             device = torch.device("cuda", torch.cuda.current_device())
